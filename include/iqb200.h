@@ -292,6 +292,130 @@ typedef struct iq_moe_down_args {
 
 int iq_moe_down(const iq_moe_down_args* a, void* stream);
 
+/* Attention of q_len new tokens a sequence over a paged key/value cache: what stands between
+ * iq_qkv_heads, which writes the caches, and iq_linear (o_proj), which reads `out`.
+ *
+ * Row j of sequence b lies in row page_table[b][j / page_size] * page_size + j % page_size of
+ * the caches ([capacity, kv_heads, head_dim], bf16 or e4m3; iq_qkv_heads writes them).
+ * lengths[b] counts the rows, the new tokens' among them: row r of the step is at n - q_len +
+ * r (n = lengths[b]) and sees the rows in (that - window, that], or all up to it with window
+ * 0.  out = softmax(scale q.k) v per query head (q_heads / kv_heads of them share a key/value
+ * head), lse = log of the softmax's sum; a row that sees nothing (a sequence of fewer than
+ * q_len rows, an empty one) gets zeros and -infinity.  Rows outside a query row's view never
+ * reach it, infinities and NaNs there included; rows past lengths[b] are not read.  Softmax
+ * statistics, scores and sums are fp32; the weights enter the product with v as half
+ * precision (e4m3 caches) or bf16 (bf16 caches).
+ *
+ * With `weights`, weights[b][h][j] gains the sum of the softmax weights that the query heads
+ * and rows of key/value head h gave row j; for the step's own rows it is set to it, and
+ * positions[b][h][j] (where given) to seen[b] - n + j: `seen` counts the tokens sequence b
+ * has seen in all, which eviction leaves larger than its length.
+ *
+ * head_dim is a multiple of 16 up to 256, q_len 1..8, batch up to 1024, (q_heads / kv_heads)
+ * * q_len up to 512.  Strides are in elements; those of the caches times the element size,
+ * and the caches' addresses, are multiples of 16 bytes.  `work` (iq_attn_work_bytes, 16-byte
+ * aligned) needs no initialisation; calls that share it must be ordered.  A length outside
+ * the page table is clamped and a page outside the cache read as zeros, with IQ_ERR_ROUTE in
+ * the status word. */
+typedef struct iq_attn_args {
+  const void* q;            /* bf16 [batch, q_len, q_heads, head_dim] */
+  int64_t q_b, q_r, q_h;
+  const void* k_cache;
+  const void* v_cache;
+  int64_t k_row, k_head, v_row, v_head;
+  int kv_kind;              /* IQ_ACT_BF16 or IQ_ACT_E4M3 */
+  int capacity;             /* rows of the caches */
+  const int* page_table;    /* [batch, max_pages] */
+  int64_t table_stride;
+  int page_size, max_pages;
+  const int* lengths;       /* [batch] */
+  int batch, q_len, q_heads, kv_heads, head_dim;
+  int window;               /* 0: none */
+  float scale;
+  void* out;                /* bf16 [batch, q_len, q_heads, head_dim] */
+  int64_t o_b, o_r, o_h;
+  float* lse;               /* optional fp32 [batch, q_len, q_heads], contiguous */
+  float* weights;           /* optional fp32 [batch, kv_heads, weights_rows] */
+  int64_t w_b, w_h;
+  int weights_rows;         /* >= page_size * max_pages */
+  int* positions;           /* optional int32, same shape; with `seen` */
+  int64_t p_b, p_h;
+  const int* seen;          /* [batch] */
+  void* work;
+  size_t work_bytes;
+  int* status;              /* optional device status word */
+  int pdl;
+} iq_attn_args;
+
+/* Bytes of `work` for these sizes (rows = page_size * max_pages); 0 for unsupported ones. */
+size_t iq_attn_work_bytes(int batch, int q_len, int q_heads, int kv_heads, int head_dim, int rows,
+                          int weights);
+int iq_attn_decode(const iq_attn_args* a, void* stream);
+
+/* Eviction from the paged cache by accumulated attention weight.  Per sequence b and key/value
+ * head h with n = lengths[b] > budget rows, `budget` rows stay: first the protected ones
+ * (position < keep_first, or >= seen[b] - keep_last), then those of the largest weight, ties
+ * to the lower row (a NaN weight counts as the lowest).  The rows that stay and lie below
+ * `budget` keep their place; the others move into the freed places below it, the i-th such
+ * row (ascending) into the i-th place.  K and V move in place; weights and positions of the
+ * rows that stay go to weights_out / positions_out (which may be weights / positions
+ * themselves), entries from `budget` (or n) on are left as they were; lengths_out[b] = min(n,
+ * budget) (not `lengths`: every head reads that).  Sequences must not share pages.
+ *
+ * Strides in elements, the caches' 16-byte aligned as in iq_attn_decode; rows = page_size *
+ * max_pages up to 262144; `work` (iq_evict_work_bytes) needs no initialisation. */
+typedef struct iq_evict_args {
+  void* k_cache;
+  void* v_cache;
+  int64_t k_row, k_head, v_row, v_head;
+  int kv_kind, capacity;
+  const int* page_table;
+  int64_t table_stride;
+  int page_size, max_pages;
+  const int* lengths;
+  const int* seen;
+  const float* weights;     /* [batch, kv_heads, >= rows] */
+  int64_t w_b, w_h;
+  const int* positions;
+  int64_t p_b, p_h;
+  float* weights_out;
+  int64_t wo_b, wo_h;
+  int* positions_out;
+  int64_t po_b, po_h;
+  int* lengths_out;
+  int batch, kv_heads, head_dim;
+  int budget, keep_first, keep_last;
+  void* work;
+  size_t work_bytes;
+  int* status;
+  int pdl;
+} iq_evict_args;
+
+size_t iq_evict_work_bytes(int batch, int kv_heads, int rows);
+int iq_kv_evict(const iq_evict_args* a, void* stream);
+
+/* The cache rows and positions of the next q_len tokens of every sequence: slot[b * q_len + r]
+ * = the cache row of row lengths[b] + r (what iq_qkv_heads takes), pos[...] = seen[b] + r,
+ * lengths_out = lengths + q_len, seen_out = seen + q_len (both may be the inputs themselves).
+ * A sequence whose pages do not reach so far keeps its length and gets slots of -1, with
+ * IQ_ERR_ROUTE in the status word. */
+typedef struct iq_advance_args {
+  const int* page_table;
+  int64_t table_stride;
+  int page_size, max_pages, capacity;
+  const int* lengths;
+  const int* seen;
+  int* lengths_out;
+  int* seen_out;
+  int64_t* slot;
+  int64_t* pos;
+  int batch, q_len;
+  int* status;
+  int pdl;
+} iq_advance_args;
+
+int iq_kv_advance(const iq_advance_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,11 +9,16 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libiqb200.so")
-SOURCES = ("kernels.cu",)
-HEADERS = ("common.cuh", "stream_core.cuh", "direct.cuh", "direct_gate.cuh")
+OBJ = os.path.join(HERE, "build")
+# source -> the headers it includes (beside the C ABI's)
+SOURCES = {
+    "kernels.cu": ("common.cuh", "stream_core.cuh", "direct.cuh", "direct_gate.cuh"),
+    "attention.cu": ("common.cuh", "paged.cuh"),
+    "kv_cache.cu": ("common.cuh", "paged.cuh"),
+}
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "--expt-relaxed-constexpr", "-shared", "-Xcompiler", "-fPIC",
+    "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
 )
 
 
@@ -24,31 +29,60 @@ def _nvcc() -> str:
     return path
 
 
-def stale() -> bool:
-    if not os.path.exists(LIB):
+def _newer(target: str, deps) -> bool:
+    """Whether `target` is missing or older than one of `deps`."""
+    if not os.path.exists(target):
         return True
-    built = os.path.getmtime(LIB)
-    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
-    deps.append(os.path.join(HERE, os.pardir, "include", "iqb200.h"))
+    built = os.path.getmtime(target)
     return any(os.path.getmtime(d) > built for d in deps)
 
 
+def _deps(source: str):
+    return [os.path.join(CSRC, f) for f in (source, *SOURCES[source])] + \
+        [os.path.join(HERE, os.pardir, "include", "iqb200.h")]
+
+
+def stale() -> bool:
+    return any(_newer(LIB, _deps(s)) for s in SOURCES)
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library if it is missing or older than its sources; returns its path."""
+    """Compile the library if it is missing or older than its sources; returns its path.
+    The sources are compiled side by side, and only those older than what they include
+    (all of them with `force`)."""
     if not force and not stale():
         return LIB
-    # compile beside the target and rename: a reader never sees a half-written library
+    os.makedirs(OBJ, exist_ok=True)
+    nvcc = _nvcc()
+    objects, running = [], []
+    for source in SOURCES:
+        obj = os.path.join(OBJ, source.replace(".cu", ".o"))
+        objects.append(obj)
+        if not force and not _newer(obj, _deps(source)):
+            continue
+        cmd = [nvcc, *NVCC_FLAGS, "-c", "-o", obj + ".new", os.path.join(CSRC, source)]
+        if verbose:
+            cmd[1:1] = ["-Xptxas", "-v"]
+        running.append((obj, subprocess.Popen(cmd, stdout=subprocess.PIPE,
+                                              stderr=subprocess.STDOUT, text=True)))
+    failed = []
+    for obj, proc in running:
+        text, _ = proc.communicate()
+        if proc.returncode != 0:
+            failed.append(text)
+            continue
+        os.replace(obj + ".new", obj)
+        if verbose:
+            print(text)
+    if failed:
+        raise RuntimeError("nvcc failed:\n" + "\n".join(failed))
+    # link beside the target and rename: a reader never sees a half-written library
     staged = LIB + ".new"
-    cmd = [_nvcc(), *NVCC_FLAGS, "-o", staged, *(os.path.join(CSRC, s) for s in SOURCES)]
-    if verbose:
-        cmd.insert(1, "-Xptxas")
-        cmd.insert(2, "-v")
-    proc = subprocess.run(cmd, capture_output=True, text=True)
+    proc = subprocess.run([nvcc, *NVCC_FLAGS, "-shared", "-o", staged, *objects],
+                          capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"nvcc failed:\n{proc.stdout}\n{proc.stderr}")
     os.replace(staged, LIB)
-    if verbose:
-        print(proc.stderr)
     return LIB
 
 

@@ -16,7 +16,7 @@ ERR_NAMES = {
     IQ_OK: "ok", IQ_ERR_ARG: "bad argument", IQ_ERR_CUDA: "CUDA call failed",
     IQ_ERR_PIPE_TIMEOUT: "shared-memory pipeline wait timed out",
     IQ_ERR_PEER_TIMEOUT: "a peer rank did not arrive in time",
-    IQ_ERR_ROUTE: "expert id out of range", IQ_ERR_UNSUPPORTED: "unsupported shape",
+    IQ_ERR_ROUTE: "expert id, cache row, page or length out of range", IQ_ERR_UNSUPPORTED: "unsupported shape",
 }
 
 X_BF16_GROUPQ, X_BF16_SPLIT2, X_E4M3_GROUP, X_E4M3_UNSCALED = range(4)
@@ -26,7 +26,8 @@ ACT_E4M3, ACT_BF16 = range(2)
 
 EXPORTS = ("iq_scratch_bytes", "iq_status_read", "iq_sm_count", "iq_tail", "iq_linear",
            "iq_linear_static", "iq_linear_static_status", "iq_qkv_heads", "iq_router",
-           "iq_moe_gate", "iq_moe_down")
+           "iq_moe_gate", "iq_moe_down", "iq_attn_work_bytes", "iq_attn_decode",
+           "iq_evict_work_bytes", "iq_kv_evict", "iq_kv_advance")
 
 
 class IqError(RuntimeError):
@@ -113,6 +114,53 @@ class MoeDownArgs(C.Structure):
     ]
 
 
+class AttnArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("q_b", C.c_int64), ("q_r", C.c_int64), ("q_h", C.c_int64),
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+        ("k_row", C.c_int64), ("k_head", C.c_int64), ("v_row", C.c_int64), ("v_head", C.c_int64),
+        ("kv_kind", C.c_int), ("capacity", C.c_int),
+        ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+        ("page_size", C.c_int), ("max_pages", C.c_int), ("lengths", C.c_void_p),
+        ("batch", C.c_int), ("q_len", C.c_int), ("q_heads", C.c_int), ("kv_heads", C.c_int),
+        ("head_dim", C.c_int), ("window", C.c_int), ("scale", C.c_float),
+        ("out", C.c_void_p), ("o_b", C.c_int64), ("o_r", C.c_int64), ("o_h", C.c_int64),
+        ("lse", C.c_void_p), ("weights", C.c_void_p), ("w_b", C.c_int64), ("w_h", C.c_int64),
+        ("weights_rows", C.c_int), ("positions", C.c_void_p), ("p_b", C.c_int64),
+        ("p_h", C.c_int64), ("seen", C.c_void_p), ("work", C.c_void_p), ("work_bytes", C.c_size_t),
+        ("status", C.c_void_p), ("pdl", C.c_int),
+    ]
+
+
+class EvictArgs(C.Structure):
+    _fields_ = [
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+        ("k_row", C.c_int64), ("k_head", C.c_int64), ("v_row", C.c_int64), ("v_head", C.c_int64),
+        ("kv_kind", C.c_int), ("capacity", C.c_int),
+        ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+        ("page_size", C.c_int), ("max_pages", C.c_int),
+        ("lengths", C.c_void_p), ("seen", C.c_void_p),
+        ("weights", C.c_void_p), ("w_b", C.c_int64), ("w_h", C.c_int64),
+        ("positions", C.c_void_p), ("p_b", C.c_int64), ("p_h", C.c_int64),
+        ("weights_out", C.c_void_p), ("wo_b", C.c_int64), ("wo_h", C.c_int64),
+        ("positions_out", C.c_void_p), ("po_b", C.c_int64), ("po_h", C.c_int64),
+        ("lengths_out", C.c_void_p),
+        ("batch", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+        ("budget", C.c_int), ("keep_first", C.c_int), ("keep_last", C.c_int),
+        ("work", C.c_void_p), ("work_bytes", C.c_size_t), ("status", C.c_void_p), ("pdl", C.c_int),
+    ]
+
+
+class AdvanceArgs(C.Structure):
+    _fields_ = [
+        ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+        ("page_size", C.c_int), ("max_pages", C.c_int), ("capacity", C.c_int),
+        ("lengths", C.c_void_p), ("seen", C.c_void_p), ("lengths_out", C.c_void_p),
+        ("seen_out", C.c_void_p), ("slot", C.c_void_p), ("pos", C.c_void_p),
+        ("batch", C.c_int), ("q_len", C.c_int), ("status", C.c_void_p), ("pdl", C.c_int),
+    ]
+
+
 _LIB = None
 
 
@@ -142,12 +190,18 @@ def load() -> C.CDLL:
         lib.iq_tail.argtypes = [C.POINTER(TailArgs), C.c_void_p, C.c_int]
         for name, struct in (("iq_linear", LinearArgs), ("iq_linear_static", LinearArgs),
                              ("iq_qkv_heads", HeadsArgs), ("iq_router", RouterArgs),
-                             ("iq_moe_gate", MoeGateArgs), ("iq_moe_down", MoeDownArgs)):
+                             ("iq_moe_gate", MoeGateArgs), ("iq_moe_down", MoeDownArgs),
+                             ("iq_attn_decode", AttnArgs), ("iq_kv_evict", EvictArgs),
+                             ("iq_kv_advance", AdvanceArgs)):
             fn = getattr(lib, name)
             fn.restype = C.c_int
             fn.argtypes = [C.POINTER(struct), C.c_void_p]
         lib.iq_linear_static_status.restype = C.c_int
         lib.iq_linear_static_status.argtypes = [C.POINTER(C.c_int), C.c_void_p]
+        lib.iq_attn_work_bytes.restype = C.c_size_t
+        lib.iq_attn_work_bytes.argtypes = [C.c_int] * 7
+        lib.iq_evict_work_bytes.restype = C.c_size_t
+        lib.iq_evict_work_bytes.argtypes = [C.c_int] * 3
         _LIB = lib
     return _LIB
 

@@ -21,6 +21,7 @@ E4M3 = torch.float8_e4m3fn
 __all__ = ["Scratch", "TailSpec", "linear", "linear_static", "linear_static_status", "qkv_heads",
            "router",
            "moe_gate", "moe_down", "tail",
+           "AttnWork", "attn_decode", "EvictWork", "kv_evict", "kv_advance",
            "X_BF16_GROUPQ", "X_BF16_SPLIT2", "X_E4M3_GROUP", "X_E4M3_UNSCALED",
            "TAIL_ATTN", "TAIL_MLP", "ROUTE_SOFTMAX", "ROUTE_SIGMOID", "ACT_E4M3", "ACT_BF16"]
 
@@ -387,3 +388,269 @@ def linear_static_status() -> int:
     _lib.check("iq_linear_static_status",
                _lib.load().iq_linear_static_status(C.byref(code), _stream()))
     return code.value
+
+
+# ---------------------------------------------------------------------- the paged KV cache
+def _gpu(name, t):
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor, got {t.device}")
+
+
+def _on(dev, name, args):
+    """Calls entry point `name` on `dev`'s current stream, with `dev` as the current device."""
+    fn = getattr(_lib.load(), name)
+    if dev.index == torch.cuda.current_device():
+        _lib.check(name, fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            _lib.check(name, fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream))
+
+
+def _strided(name, t, dtype, shape, dev, written=False):
+    """Checks a tensor whose last axis is contiguous (others may have any stride, no two
+    elements at one address where it is `written`); returns its strides."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must have dtype {dtype}, got {t.dtype}")
+    if t.device != dev:
+        raise ValueError(f"{name} must be on {dev}, got {t.device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    st = t.stride()
+    if st[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"{name} must be contiguous along its last axis")
+    if written and not t.is_contiguous():
+        reach = 1
+        for size, step in sorted(zip(shape, st), key=lambda x: x[1]):
+            if size > 1:
+                if step < reach:
+                    raise ValueError(f"{name} must not overlap itself (strides {st})")
+                reach = step * (size - 1) + reach
+    return st
+
+
+def _cache_pair(k_cache, v_cache, dev, written=False):
+    if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 3:
+        raise ValueError("the KV caches must be [capacity, kv_heads, head_dim] tensors")
+    if k_cache.dtype != torch.bfloat16 and k_cache.dtype != E4M3:
+        raise ValueError("the KV caches must both be bf16 or both e4m3")
+    ks = _strided("k_cache", k_cache, k_cache.dtype, k_cache.shape, dev, written)
+    vs = _strided("v_cache", v_cache, k_cache.dtype, k_cache.shape, dev, written)
+    return ks, vs
+
+
+def _paging(a, page_table, page_size, batch, dev):
+    st = _strided("page_table", page_table, torch.int32, page_table.shape, dev)
+    if page_table.dim() != 2 or page_table.shape[0] != batch or page_table.shape[1] < 1:
+        raise ValueError(f"page_table must be [{batch}, pages >= 1], got "
+                         f"{tuple(page_table.shape)}")
+    if page_size < 1:
+        raise ValueError(f"page_size must be at least 1, got {page_size}")
+    a.page_table, a.table_stride = page_table.data_ptr(), st[0]
+    a.page_size, a.max_pages = page_size, page_table.shape[1]
+    return page_size * page_table.shape[1]
+
+
+class AttnWork:
+    """The work area of `attn_decode` for given sizes (`rows`: page_size x pages of the page
+    table; `weights`: for calls that accumulate weights).  Calls that share one must be
+    ordered on one stream, replays of graphs that captured it included."""
+
+    def __init__(self, *, batch: int, q_len: int, q_heads: int, kv_heads: int, head_dim: int,
+                 rows: int, weights: bool = False, device="cuda"):
+        self.bytes = int(_lib.load().iq_attn_work_bytes(batch, q_len, q_heads, kv_heads, head_dim,
+                                                        rows, int(weights)))
+        if self.bytes == 0:
+            raise ValueError(
+                f"unsupported attention shape: batch {batch}, q_len {q_len}, heads {q_heads}/"
+                f"{kv_heads}, head_dim {head_dim}, rows {rows} (head_dim a multiple of 16 up to "
+                "256, q_len 1..8, batch up to 1024, q_heads a multiple of kv_heads and at most "
+                "512 query rows a key/value head)")
+        self.buf = torch.empty(self.bytes, dtype=torch.uint8, device=device)
+        self.ptr = self.buf.data_ptr()
+
+
+def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, scale=None,
+                window: int = 0, out=None, lse=None, weights=None, positions=None, seen=None,
+                work: AttnWork | None = None, scratch: Scratch | None = None, pdl: bool = False):
+    """Attention of the last `q_len` tokens of each sequence over its paged KV cache
+    (`iq_attn_decode`): `q [batch, q_len, q_heads, D]` bf16 -> `out`, same shape.
+
+    `k_cache` / `v_cache [capacity, kv_heads, D]` are what `qkv_heads` writes (bf16 or e4m3),
+    row j of sequence b being row `page_table[b, j // page_size] * page_size + j % page_size`;
+    `lengths [batch]` (int32) counts the rows with the new ones.  New token r sees the rows up
+    to its own, the last `window` of them if `window` is not 0.  A token that sees nothing
+    gets zeros, and -inf in `lse [batch, q_len, q_heads]` (fp32, optional).  `scale` defaults
+    to D ** -0.5.
+
+    `weights [batch, kv_heads, >= rows]` (fp32) gains each row's softmax weights, summed over
+    the query heads of its key/value head and the new tokens; the new tokens' own entries are
+    set, and those of `positions` (int32, same shape) to the tokens' positions, `seen [batch]`
+    (int32) being the tokens seen so far with the new ones.  Without `work` one is allocated
+    for the call.  A length or page out of range shows in `scratch`'s status word."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 4:
+        raise ValueError("q must be a tensor [batch, q_len, q_heads, head_dim]")
+    dev, shape = q.device, q.shape
+    batch, q_len, q_heads, d = shape
+    a = _lib.AttnArgs()
+    qs = _strided("q", q, torch.bfloat16, shape, dev)
+    ks, vs = _cache_pair(k_cache, v_cache, dev)
+    capacity, kv_heads, kd = k_cache.shape
+    if kd != d or kv_heads < 1 or q_heads % kv_heads:
+        raise ValueError(f"q {tuple(shape)} does not fit caches of {kv_heads} heads of {kd}")
+    rows = _paging(a, page_table, page_size, batch, dev)
+    _strided("lengths", lengths, torch.int32, (batch,), dev)
+    if window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    os_ = _strided("out", out, torch.bfloat16, shape, dev, True)
+    if lse is not None:
+        _strided("lse", lse, torch.float32, shape[:3], dev)
+        if not lse.is_contiguous():
+            raise ValueError("lse must be contiguous")
+        a.lse = lse.data_ptr()
+    if weights is not None:
+        if weights.dim() != 3 or weights.shape[2] < rows:
+            raise ValueError(f"weights must be [{batch}, {kv_heads}, >= {rows}], got "
+                             f"{tuple(weights.shape)}")
+        n = weights.shape[2]
+        ws = _strided("weights", weights, torch.float32, (batch, kv_heads, n), dev, True)
+        a.weights, a.w_b, a.w_h, a.weights_rows = weights.data_ptr(), ws[0], ws[1], n
+    if (positions is None) != (seen is None) or (positions is not None and weights is None):
+        raise ValueError("positions and seen come together, with weights")
+    if positions is not None:
+        ps = _strided("positions", positions, torch.int32, weights.shape, dev, True)
+        _strided("seen", seen, torch.int32, (batch,), dev)
+        a.positions, a.p_b, a.p_h, a.seen = positions.data_ptr(), ps[0], ps[1], seen.data_ptr()
+    _gpu("q", q)
+    if work is None:
+        work = AttnWork(batch=batch, q_len=q_len, q_heads=q_heads, kv_heads=kv_heads, head_dim=d,
+                        rows=rows, weights=weights is not None, device=dev)
+    elif work.buf.device != dev:
+        raise ValueError(f"work must be on {dev}, got {work.buf.device}")
+    a.q, a.q_b, a.q_r, a.q_h = q.data_ptr(), qs[0], qs[1], qs[2]
+    a.k_cache, a.k_row, a.k_head = k_cache.data_ptr(), ks[0], ks[1]
+    a.v_cache, a.v_row, a.v_head = v_cache.data_ptr(), vs[0], vs[1]
+    a.kv_kind = ACT_E4M3 if k_cache.dtype == E4M3 else ACT_BF16
+    a.capacity, a.lengths = capacity, lengths.data_ptr()
+    a.batch, a.q_len, a.q_heads, a.kv_heads, a.head_dim = batch, q_len, q_heads, kv_heads, d
+    a.window, a.scale = window, d ** -0.5 if scale is None else scale
+    a.out, a.o_b, a.o_r, a.o_h = out.data_ptr(), os_[0], os_[1], os_[2]
+    a.work, a.work_bytes = work.ptr, work.bytes
+    if scratch is not None:
+        a.status = scratch.ptr
+    a.pdl = int(pdl)
+    _on(dev, "iq_attn_decode", a)
+    return out
+
+
+class EvictWork:
+    """The work area of `kv_evict` for given sizes (`rows`: page_size x pages of the page
+    table).  Calls that share one must be ordered on one stream."""
+
+    def __init__(self, *, batch: int, kv_heads: int, rows: int, device="cuda"):
+        self.bytes = int(_lib.load().iq_evict_work_bytes(batch, kv_heads, rows))
+        if self.bytes == 0:
+            raise ValueError(f"unsupported eviction shape: batch {batch}, {kv_heads} heads, {rows} "
+                             "rows (batch x heads up to 65535, rows up to 262144)")
+        self.buf = torch.empty(self.bytes, dtype=torch.uint8, device=device)
+        self.ptr = self.buf.data_ptr()
+
+
+def kv_evict(k_cache, v_cache, page_table, lengths, weights, positions, seen, *, page_size: int,
+             budget: int, lengths_out, keep_first: int = 0, keep_last: int = 0, weights_out=None,
+             positions_out=None, work: EvictWork | None = None, scratch: Scratch | None = None,
+             pdl: bool = False):
+    """Cuts every sequence of more than `budget` rows down to `budget` (`iq_kv_evict`): each
+    key/value head keeps its rows of position < `keep_first` or >= `seen - keep_last`, then
+    those of the largest accumulated weight (ties to the lower row).
+
+    `weights` (fp32) and `positions` (int32) are `[batch, kv_heads, >= rows]` as `attn_decode`
+    keeps them.  Rows that stay below `budget` stay where they are; the others move, in place
+    and in ascending order, into the places freed there, with their weights and positions
+    (`weights_out` / `positions_out`, by default the inputs themselves).  `lengths_out [batch]`
+    (int32, not `lengths`: layers of a model share the lengths of before) gets the new
+    lengths.  Sequences must not share pages."""
+    if not isinstance(weights, torch.Tensor) or weights.dim() != 3:
+        raise ValueError("weights must be a tensor [batch, kv_heads, rows]")
+    dev = weights.device
+    batch, kv_heads, n = weights.shape
+    a = _lib.EvictArgs()
+    ks, vs = _cache_pair(k_cache, v_cache, dev, True)
+    capacity, kh, d = k_cache.shape
+    rows = _paging(a, page_table, page_size, batch, dev)
+    if kh != kv_heads or n < rows:
+        raise ValueError(f"weights must be [{batch}, {kh}, >= {rows}], got {tuple(weights.shape)}")
+    if budget < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget:
+        raise ValueError(f"budget must be at least 1 and hold the protected rows, got {budget} for "
+                         f"{keep_first} + {keep_last}")
+    weights_out = weights if weights_out is None else weights_out
+    positions_out = positions if positions_out is None else positions_out
+    ws = _strided("weights", weights, torch.float32, weights.shape, dev)
+    ps = _strided("positions", positions, torch.int32, weights.shape, dev)
+    wo = _strided("weights_out", weights_out, torch.float32, weights.shape, dev, True)
+    po = _strided("positions_out", positions_out, torch.int32, weights.shape, dev, True)
+    for name, t in (("lengths", lengths), ("seen", seen), ("lengths_out", lengths_out)):
+        _strided(name, t, torch.int32, (batch,), dev)
+    if lengths_out.data_ptr() == lengths.data_ptr():
+        raise ValueError("lengths_out must not be lengths")
+    _gpu("weights", weights)
+    if work is None:
+        work = EvictWork(batch=batch, kv_heads=kv_heads, rows=rows, device=dev)
+    elif work.buf.device != dev:
+        raise ValueError(f"work must be on {dev}, got {work.buf.device}")
+    a.k_cache, a.k_row, a.k_head = k_cache.data_ptr(), ks[0], ks[1]
+    a.v_cache, a.v_row, a.v_head = v_cache.data_ptr(), vs[0], vs[1]
+    a.kv_kind = ACT_E4M3 if k_cache.dtype == E4M3 else ACT_BF16
+    a.capacity, a.lengths, a.seen = capacity, lengths.data_ptr(), seen.data_ptr()
+    a.weights, a.w_b, a.w_h = weights.data_ptr(), ws[0], ws[1]
+    a.positions, a.p_b, a.p_h = positions.data_ptr(), ps[0], ps[1]
+    a.weights_out, a.wo_b, a.wo_h = weights_out.data_ptr(), wo[0], wo[1]
+    a.positions_out, a.po_b, a.po_h = positions_out.data_ptr(), po[0], po[1]
+    a.lengths_out = lengths_out.data_ptr()
+    a.batch, a.kv_heads, a.head_dim = batch, kv_heads, d
+    a.budget, a.keep_first, a.keep_last = budget, keep_first, keep_last
+    a.work, a.work_bytes = work.ptr, work.bytes
+    if scratch is not None:
+        a.status = scratch.ptr
+    a.pdl = int(pdl)
+    _on(dev, "iq_kv_evict", a)
+    return lengths_out
+
+
+def kv_advance(page_table, lengths, seen, slot, pos, *, page_size: int, capacity: int,
+               q_len: int = 1, lengths_out=None, seen_out=None, scratch: Scratch | None = None,
+               pdl: bool = False):
+    """The cache rows and positions of the next `q_len` tokens of every sequence
+    (`iq_kv_advance`), on the device, so that a captured step finds its own rows: `slot` and
+    `pos [batch * q_len]` (int64) are what `qkv_heads` and the rotary tables take.  `lengths`
+    and `seen [batch]` (int32) grow by `q_len`, in place unless `lengths_out` / `seen_out` are
+    given.  A sequence whose pages end before gets slots of -1, which `qkv_heads` refuses to
+    write, and stays as it was (with `scratch`'s status word set)."""
+    if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:
+        raise ValueError("lengths must be a tensor [batch]")
+    dev, batch = lengths.device, lengths.shape[0]
+    if not 1 <= q_len <= 8:
+        raise ValueError(f"q_len must be 1..8, got {q_len}")
+    if batch < 1 or capacity < 1:
+        raise ValueError("batch and capacity must be at least 1")
+    a = _lib.AdvanceArgs()
+    _paging(a, page_table, page_size, batch, dev)
+    lengths_out = lengths if lengths_out is None else lengths_out
+    seen_out = seen if seen_out is None else seen_out
+    for name, t in (("lengths", lengths), ("seen", seen), ("lengths_out", lengths_out),
+                    ("seen_out", seen_out)):
+        _strided(name, t, torch.int32, (batch,), dev)
+    for name, t in (("slot", slot), ("pos", pos)):
+        _strided(name, t, torch.int64, (batch * q_len,), dev)
+    _gpu("lengths", lengths)
+    a.capacity, a.lengths, a.seen = capacity, lengths.data_ptr(), seen.data_ptr()
+    a.lengths_out, a.seen_out = lengths_out.data_ptr(), seen_out.data_ptr()
+    a.slot, a.pos, a.batch, a.q_len = slot.data_ptr(), pos.data_ptr(), batch, q_len
+    if scratch is not None:
+        a.status = scratch.ptr
+    a.pdl = int(pdl)
+    _on(dev, "iq_kv_advance", a)
+    return slot, pos

@@ -10,23 +10,32 @@
 // head, and all the query rows that share a key/value head (group x q_len of them) use what
 // was read: HBM, until about 32 rows share a head.
 //
-// Split.  The keys every row of a step sees ("common" keys) are cut into tiles of TK; the
-// tiles of all (sequence, head, block of query rows) units form one list that is dealt to
-// the CTAs in equal contiguous shares, whatever the lengths are.  A unit that falls into
-// one share is finished there; one that spans several leaves partial results that
-// attn_join_kernel adds.  The at most 14 "edge" keys that only some rows of a step see (the
-// step's own keys, and the rim of a sliding window) are one more tile of the unit, done in
-// scalar arithmetic on exactly the visible keys: a value that a row must not see (an
-// infinity or a NaN among them) never meets that row, not even multiplied by zero.
+// Split.  A unit is a sequence, a group of HG key/value heads and a block of query rows; its
+// keys are cut into tiles of TK.  The tiles of all units form one list that is dealt to the
+// CTAs in equal contiguous shares, whatever the lengths are.  A unit that falls into one
+// share is finished there; one that spans several leaves partial results that
+// attn_join_kernel adds.  The HG heads of a group are neighbours in memory and are read at the
+// same time by the warps of one CTA, so that DRAM sees pieces of HG rows, not of one.
+//
+// What a row must not see (later tokens of its step, keys that slid out of its window, rows
+// past the end) never meets it: its score is replaced, and its value, which the product
+// would multiply by zero, is zeroed in shared memory where it is outside the unit or, for the
+// few keys that only some rows see, where it is not finite (0 x NaN); those rows then get the
+// infinities and NaNs they do see added at the end.
 //
 // Layout.  S^T = K Q^T and O^T = V^T P^T on the warp MMA (m16n8k16): the cache is the
 // 16-row operand and eight query rows the columns, so a group of eight heads fills the
-// tile that would otherwise be padded to sixteen rows.  A warp owns the sixteen keys it
-// copied (cp.async ring, no block barrier in the loop) and all of D; warps join at the end
-// of a unit.
+// tile that would otherwise be padded to sixteen rows.  A warp (with more than sixteen
+// query rows: a group of warps) owns KPW keys of a tile and all of D, with a ring of its own
+// that tiled TMA copies fill (128-byte swizzle; one box a page piece); there is no block
+// barrier in the loop, and the warps' keys join at the end of a unit.  Keys sit at absolute
+// multiples of KPW, so that a box never leaves its page; the rows of a box that lie outside
+// the common keys get no weight, and their values are zeroed in shared memory first.
 #include <math.h>
 #include <stdio.h>
 
+#include <atomic>
+#include <type_traits>
 #include <mutex>
 #include <unordered_set>
 
@@ -37,11 +46,12 @@
 namespace iqb {
 
 constexpr int kAttnMaxBatch = 1024;
-constexpr int kEdgeMax = 16;
+constexpr int kCopyThreads = 128;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnParams {
+  CUtensorMap k_map, v_map;                      // bytes: (head_dim, capacity, kv_heads)
   const __nv_bfloat16* q;
   long long q_b, q_r, q_h;                       // strides, elements
   const uint8_t *k, *v;
@@ -52,8 +62,8 @@ struct AttnParams {
   __nv_bfloat16* out;
   long long o_b, o_r, o_h;
   float* lse;                                    // [batch, q_len, q_heads] or null
-  float* part;                                   // [2 grid][RB][DP] unnormalised O
-  float2* part_ml;                               // [2 grid][RB] (M, l)
+  float* part;                                   // [2 grid][HG][RB][DP] unnormalised O
+  float2* part_ml;                               // [2 grid][HG][RB] (M, l)
   int2* units;                                   // [units] first and last CTA of a split unit
   float* scores;                                 // [batch * kv_heads][score_rows][rows_all] x_j, or null
   float* lse2;                                   // [batch, q_len, q_heads] M + log2 l (with scores)
@@ -68,27 +78,27 @@ struct AttnParams {
   int rows_all;                                  // group * q_len
   int rows_pad;                                  // rows_all rounded up to eight
   int n_rb;                                      // blocks of RB rows
+  int box_rows, box_heads;                       // of a TMA copy: divide a page and KPW; 1 or HG
+  int gather;                                    // copy by threads, 16 bytes at a time, instead
   float scale_log2;
 };
 
-// One sequence's keys: common [lo, hi), edges [lo0, lo) and [hi, n) (hi clamped to lo).
+// One sequence's keys: [lo, n) are seen by some row of the step, [lo_all, hi_all) by all.
 struct SeqSpan {
-  int n, lo0, lo, hi;
+  int n, lo, lo_all, hi_all;
 };
 __device__ __forceinline__ SeqSpan seq_span(int n, int q_len, int window) {
   SeqSpan s;
   s.n = n;
-  const int first = n - q_len;                   // the first row's position
-  s.lo0 = window ? max(0, first - window + 1) : 0;
-  s.lo = window ? max(0, n - window) : 0;
-  s.hi = max(first + 1, 0);
-  s.hi = max(s.hi, s.lo);
+  s.lo = window ? max(0, n - q_len - window + 1) : 0;
+  s.lo_all = window ? max(0, n - window) : 0;
+  s.hi_all = max(n - q_len + 1, 0);
   return s;
 }
-__device__ __forceinline__ int span_edges(const SeqSpan& s) { return s.lo - s.lo0 + s.n - s.hi; }
-template <int TK>
+// Tiles start at `lo` rounded down to the keys a warp copies.
+template <class G>
 __device__ __forceinline__ int span_tiles(const SeqSpan& s) {
-  return (s.hi - s.lo + TK - 1) / TK + (span_edges(s) > 0 ? 1 : 0);
+  return (s.n - s.lo / G::KPW * G::KPW + G::TK - 1) / G::TK;
 }
 
 __device__ __forceinline__ int clamp_length(const AttnParams& p, int b, bool report) {
@@ -100,21 +110,20 @@ __device__ __forceinline__ int clamp_length(const AttnParams& p, int b, bool rep
   return n;
 }
 
-// floor(total c / grid), and the share that owns tile i.
-__device__ __forceinline__ int share_begin(int total, int grid, int c) {
-  return static_cast<int>(static_cast<long long>(total) * c / grid);
-}
-__device__ __forceinline__ int share_owner(int total, int grid, int i) {
-  return static_cast<int>((static_cast<long long>(i + 1) * grid - 1) / total);
-}
-
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+// D(16x8, fp32) += A(16x16) B(16x8), operands half (e4m3 caches) or bf16.
+template <int KV>
+__device__ __forceinline__ void mma_k16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
-      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  if (KV == IQ_ACT_BF16)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
   uint32_t h;
@@ -146,6 +155,14 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
                : "r"(addr)
                : "memory");
 }
+__device__ __forceinline__ void tma_3d_g2s(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
+                                           uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
@@ -153,87 +170,208 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
 }
 
 // KV: IQ_ACT_E4M3 or IQ_ACT_BF16.  DP: head dim rounded up (64, 128, 256).  NBW: blocks of
-// eight query rows a warp holds; WR: warps that share a key group's copies, each with its
-// own rows; W warps.
-template <int KV_, int DP_, int NBW_, int WR_, int W_, int CTAS_>
+// eight query rows a warp holds; WR warps share a head's keys, each with its own rows; HG
+// heads a unit; W warps that compute.  The W / WR / HG = KG groups of warps have a ring each,
+// of stages of KPW keys of all HG heads; KPW is what makes a stage of all rings 64 KB.
+template <int KV_, int DP_, int NBW_, int WR_, int HG_, int W_>
 struct AttnGeo {
-  static constexpr int KV = KV_, DP = DP_, NBW = NBW_, WR = WR_, W = W_, CTAS = CTAS_;
-  static constexpr int WK = W / WR;
-  static constexpr int TK = 16 * WK;             // keys a tile
-  static constexpr int RB = 8 * NBW * WR;        // query rows a block
-  static constexpr int THREADS = 32 * W;
+  static constexpr int KV = KV_, DP = DP_, NBW = NBW_, WR = WR_, HG = HG_, W = W_;
   static constexpr int ELT = KV == IQ_ACT_BF16 ? 2 : 1;
   static constexpr int DPB = DP * ELT;
-  static constexpr int CPR = DPB / 16;           // 16-byte pieces a row
-  static constexpr int STAGE = 2 * 16 * DPB;     // one key group's keys and values
+  static constexpr int WK = W / WR;
+  static constexpr int KG = WK / HG;
+  static constexpr int KPW = 32768 / (WK * DPB) < 16 ? 16 : 32768 / (WK * DPB);
+  static constexpr int SUB = KPW / 16;
+  static constexpr int SUBI = SUB > 1 ? 2 : 1;   // tiles of sixteen keys in flight together
+  static constexpr int TK = KPW * KG;            // keys a tile
+  static constexpr int RB = 8 * NBW * WR;        // query rows a block
+  static constexpr int CONSUMERS = 32 * W;
+  static constexpr int THREADS = CONSUMERS + kCopyThreads;
+  // Registers move from the copying warps to the others (eight of those: 12 warps share the
+  // file at 168 a thread; the shares add up to what the block was launched with)
+  static constexpr bool MOVE_REGS = W == 8;
+  static constexpr int REGS = 168, REGS_COPY = 72, REGS_COMPUTE = 216;
+  static_assert(REGS_COPY * kCopyThreads + REGS_COMPUTE * CONSUMERS <= REGS * THREADS || !MOVE_REGS,
+                "the register shares are those of the launch");
+  static constexpr int PITCH = DPB < 128 ? DPB : 128;   // bytes of a row in one box
+  static constexpr int BOXES = DPB / PITCH;      // boxes side by side that make a row
+  static constexpr int HEAD = KPW * PITCH;       // one head of one box
+  static constexpr int BOX = HG * HEAD;          // a stage: [keys, values][box][head][row]
+  static constexpr int HALF = BOXES * BOX;
+  static constexpr int STAGE = 2 * HALF;
   static constexpr int MT = DP / 16;             // m-tiles of O^T
-  static constexpr int NREG = MT * 4 + 4;      // one block of eight rows: O, M, l of a lane
-  static constexpr int TREE = WK > 1 ? (W / 2) * 32 * NREG * 4 : 0;
-  static constexpr int EDGE = RB * (DP + 2) * 4;
-  static constexpr int JOIN = TREE > EDGE ? TREE : EDGE;
-  static constexpr int FIXED = JOIN + kEdgeMax * 4 + (2 * kAttnMaxBatch + 64) * 4;
-  static constexpr int BUDGET = (CTAS == 1 ? 227 : CTAS == 2 ? 113 : 75) * 1024;
-  static constexpr int FIT = (BUDGET - FIXED) / (WK * STAGE);
-  static constexpr int STAGES = FIT > 8 ? 8 : FIT;
-  static constexpr int SMEM = WK * STAGES * STAGE + FIXED;
+  static constexpr int QREG = DP / 8;            // packed registers of q a block of eight rows
+  static constexpr bool QS = NBW * DP >= 512;    // q's fragments live in shared memory
+  // joining warps exchange one block of eight rows: a lane's M, l and O, in XP parts
+  static constexpr int XP = W == 16 ? 2 : 1;
+  static constexpr int NREG = MT / XP * 4 + 4;
+  static constexpr int JOIN = KG > 1 ? (W / 2) * 32 * NREG * 4 : 0;
+  static constexpr int QBYTES = QS ? HG * WR * NBW * QREG * 128 : 0;
+  static constexpr int MAX_STAGES = 8;
+  static constexpr int FIXED = 1024 + JOIN + QBYTES + 2 * KG * MAX_STAGES * 8 + (2 * kAttnMaxBatch + 64) * 4;
+  static constexpr int FIT = (227 * 1024 - FIXED) / (KG * STAGE);
+  static constexpr int STAGES = FIT > MAX_STAGES ? MAX_STAGES : FIT;
+  static constexpr int SMEM = KG * STAGES * STAGE + FIXED;
   static_assert(STAGES >= 2, "the ring needs two stages");
+  static_assert(HEAD % 1024 == 0, "swizzled boxes start on their pattern's period");
+  static_assert(KPW <= 256, "a box has at most 256 rows");
+  static_assert(WK % HG == 0, "every head has the same number of rings");
 };
 
-// Walks the list of tiles: the unit of the current tile and the tile's place in it.
-struct TileIter {
-  int b, hb, tile, tiles;
-  SeqSpan s;
-};
-
+// The key of a sixteen-key tile that sits in row i (of eight) of the MMA operand.  e4m3: a
+// permutation under which the 16-byte (8-byte at D = 64) loads of both the keys' and the
+// values' fragments touch every bank once on rows that TMA swizzled.  bf16 (ldmatrix): none.
 template <class G>
-__device__ __forceinline__ void iter_seq(TileIter& it, const AttnParams& p, const int* prefix,
-                                         const int* lens) {
-  it.tiles = prefix[it.b + 1] - prefix[it.b];
-  it.s = seq_span(lens[it.b], p.q_len, p.window);
+__device__ __forceinline__ int key_of(int i) {
+  if (G::KV == IQ_ACT_BF16) return i;
+  if (G::DPB >= 128) return i & 1 ? i ^ 4 : i;   // 0 5 2 7 4 1 6 3
+  return (0x65742130 >> (4 * i)) & 7;            // 0 3 1 2 4 7 5 6
 }
+// Byte offset of 16-byte piece c of row r inside a box.
 template <class G>
-__device__ __forceinline__ void iter_init(TileIter& it, const AttnParams& p, const int* prefix,
-                                          const int* lens, int i) {
-  const int per = p.kv_heads * p.n_rb;
-  int lo = 0, hi = p.batch;                      // prefix[lo] * per <= i < prefix[hi] * per
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (prefix[mid] * per <= i) lo = mid; else hi = mid;
+__device__ __forceinline__ int swizzled(int r, int c) {
+  return G::PITCH == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+}
+// The channel of rows g (y = 0) and g + 8 (y = 1) of m-tile x of O^T.
+template <class G>
+__device__ __forceinline__ int channel_of(int x, int y, int g) {
+  if (G::KV == IQ_ACT_BF16) return 16 * x + 8 * y + g;
+  return G::DP >= 128 ? (x / 8) * 128 + g * 16 + 2 * (x % 8) + y : g * 8 + 2 * x + y;
+}
+
+// A place in the list of tiles.
+template <class G>
+struct Walk {
+  int b, hb;                                     // sequence; head group and block of rows
+  int left;                                      // tiles of the unit from here on
+  int j;                                         // the tile's first key
+  int lo, n;                                     // the unit's keys
+  int h0, r0;                                    // first head, first query row
+
+  __device__ __forceinline__ void unit(const AttnParams& p, const int* prefix, const int* lens, int tile) {
+    const SeqSpan s = seq_span(lens[b], p.q_len, p.window);
+    lo = s.lo;
+    n = s.n;
+    left = prefix[b + 1] - prefix[b] - tile;
+    j = s.lo / G::KPW * G::KPW + tile * G::TK;
+    const int hg = p.n_rb == 1 ? hb : hb / p.n_rb;
+    h0 = hg * G::HG;
+    r0 = (hb - hg * p.n_rb) * G::RB;
   }
-  it.b = lo;
-  iter_seq<G>(it, p, prefix, lens);
-  const int rem = i - prefix[lo] * per;
-  it.hb = rem / it.tiles;
-  it.tile = rem - it.hb * it.tiles;
+  // Returns the tile's place in its unit.
+  __device__ __forceinline__ int start(const AttnParams& p, const int* prefix, const int* lens, int per, int i) {
+    int first = 0, end = p.batch;                // prefix[first] * per <= i < prefix[end] * per
+    while (end - first > 1) {
+      const int mid = (first + end) >> 1;
+      if (prefix[mid] * per <= i) first = mid; else end = mid;
+    }
+    b = first;
+    const int tiles = prefix[b + 1] - prefix[b], rem = i - prefix[b] * per;
+    hb = rem / tiles;
+    unit(p, prefix, lens, rem - hb * tiles);
+    return rem - hb * tiles;
+  }
+  __device__ __forceinline__ void next(const AttnParams& p, const int* prefix, const int* lens, int per) {
+    j += G::TK;
+    if (--left > 0) return;
+    if (++hb == per) {
+      hb = 0;
+      do {
+        if (++b == p.batch) return;
+      } while (prefix[b + 1] == prefix[b]);
+    }
+    unit(p, prefix, lens, 0);
+  }
+};
+
+// Zeroes what is not finite among sixteen bytes of values; whether there was any.
+template <int KV>
+__device__ __forceinline__ bool strip(uint4& v) {
+  uint32_t* w = &v.x;
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (KV == IQ_ACT_BF16) {
+#pragma unroll
+      for (int x = 0; x < 32; x += 16)
+        if ((w[i] >> x & 0x7f80u) == 0x7f80u) { w[i] &= ~(0xffffu << x); any = true; }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 32; x += 8)
+        if ((w[i] >> x & 0x7fu) == 0x7fu) { w[i] &= ~(0xffu << x); any = true; }
+    }
+  }
+  return any;
 }
+
+// Adds to the segment's results, which its warps have just written (to `out`, or to partial
+// results `slot`), the infinities and NaNs that `strip` took out of the values of the keys
+// [from, to) that only some rows see.  (Their weight is positive, so it does not matter.)
+// All consumer threads of the CTA call it.
 template <class G>
-__device__ __forceinline__ void iter_next(TileIter& it, const AttnParams& p, const int* prefix,
-                                          const int* lens) {
-  if (++it.tile < it.tiles) return;
-  it.tile = 0;
-  if (++it.hb < p.kv_heads * p.n_rb) return;
-  it.hb = 0;
-  do {
-    ++it.b;
-  } while (it.b < p.batch && prefix[it.b + 1] == prefix[it.b]);
-  if (it.b < p.batch) iter_seq<G>(it, p, prefix, lens);
+__device__ __noinline__ void add_not_finite(const AttnParams& p, int b, int n, int h0, int r0, int from,
+                                            int to, bool whole, int slot) {
+  const SeqSpan s = seq_span(n, p.q_len, p.window);
+  const int rows = min(G::RB, p.rows_all - r0);
+  for (int i = threadIdx.x; i < G::HG * rows * p.dim; i += G::CONSUMERS) {
+    const int d = i % p.dim, rr = i / p.dim % rows, hg = i / p.dim / rows;
+    const int h = h0 + hg, tok = (r0 + rr) / p.group, head = h * p.group + (r0 + rr) % p.group;
+    const int pos = n - p.q_len + tok;
+    float sum = 0.f;
+    for (int j = max(from, p.window ? pos - p.window + 1 : 0); j < min(to, pos + 1); ++j) {
+      if (j < 0 || (j >= s.lo_all && j < s.hi_all)) continue;   // seen by all: in the product already
+      const int row = cache_row(p.pages, b, j);
+      if (row < 0) continue;
+      const uint8_t* v = p.v + row * p.v_row + h * p.v_head;
+      const float x = G::KV == IQ_ACT_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(v)[d])
+                                           : e4m3_to_f32(v[d]);
+      if (!isfinite(x)) sum += x;
+    }
+    if (sum == 0.f) continue;
+    if (whole) {
+      p.out[b * p.o_b + tok * p.o_r + head * p.o_h + d] = __float2bfloat16_rn(sum);
+    } else {
+      // the place of (rr, d) in the fragments
+      int x, y, g;
+      if (G::KV == IQ_ACT_BF16) { x = d / 16; y = d / 8 % 2; g = d % 8; }
+      else if (G::DP >= 128) { x = d / 128 * 8 + d % 16 / 2; y = d % 2; g = d % 128 / 16; }
+      else { x = d % 8 / 2; y = d % 2; g = d / 8; }
+      const size_t block = (static_cast<size_t>(slot) * G::HG + hg) * (G::RB / 8) + rr / 8;
+      p.part[((block * G::MT + x) * 32 + 4 * g + rr % 8 / 2) * 4 + 2 * y + rr % 2] += sum;
+    }
+  }
 }
 
 template <class G>
-__global__ void __launch_bounds__(G::THREADS, G::CTAS) attn_kernel(const __grid_constant__ AttnParams p) {
-  extern __shared__ __align__(1024) uint8_t smem[];
+__global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_constant__ AttnParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* ring = smem;
-  float* join = reinterpret_cast<float*>(smem + G::WK * G::STAGES * G::STAGE);
-  int* edge_rows = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(join) + G::JOIN);
-  int* prefix = edge_rows + kEdgeMax;            // [batch + 1]
+  float* join = reinterpret_cast<float*>(smem + G::KG * G::STAGES * G::STAGE);
+  uint32_t* q_smem = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(join) + G::JOIN);
+  uint64_t* bar_full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(q_smem) + G::QBYTES);
+  uint64_t* bar_free = bar_full + G::KG * G::MAX_STAGES;                // both [ring][stage]
+  int* prefix = reinterpret_cast<int*>(bar_free + G::KG * G::MAX_STAGES);   // [batch + 1]
   int* lens = prefix + kAttnMaxBatch + 4;        // [batch]
   int* warp_sums = lens + kAttnMaxBatch;         // [W]
+  int* not_finite = warp_sums + 32;              // a value that only some rows see is not finite
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int wr = warp % G::WR, kg = warp / G::WR;
+  // rows, head of the unit, ring
+  const int wr = warp % G::WR, hg = warp / G::WR % G::HG, kg = warp / (G::WR * G::HG);
   const int g = lane >> 2, t = lane & 3;
   const int cta = blockIdx.x;
 
+  if (tid < G::KG * G::STAGES) {
+    mbar_init(bar_full + (tid / G::STAGES) * G::MAX_STAGES + tid % G::STAGES, p.gather ? kCopyThreads : 1);
+    mbar_init(bar_free + (tid / G::STAGES) * G::MAX_STAGES + tid % G::STAGES, G::HG * G::WR);
+  }
+  mbar_fence_init();
+  if (tid == 0) {
+    *not_finite = 0;
+    prefetch_tensormap(&p.k_map);
+    prefetch_tensormap(&p.v_map);
+  }
   pdl_wait();
   pdl_launch_dependents();
 
@@ -242,10 +380,11 @@ __global__ void __launch_bounds__(G::THREADS, G::CTAS) attn_kernel(const __grid_
     const int each = (p.batch + G::THREADS - 1) / G::THREADS;
     const int b0 = min(tid * each, p.batch), b1 = min(b0 + each, p.batch);
     int sum = 0;
+#pragma unroll 1
     for (int b = b0; b < b1; ++b) {
       const int n = clamp_length(p, b, cta == 0);
       lens[b] = n;
-      sum += span_tiles<G::TK>(seq_span(n, p.q_len, p.window));
+      sum += span_tiles<G>(seq_span(n, p.q_len, p.window));
     }
     int incl = sum;
 #pragma unroll
@@ -256,38 +395,158 @@ __global__ void __launch_bounds__(G::THREADS, G::CTAS) attn_kernel(const __grid_
     if (lane == 31) warp_sums[warp] = incl;
     __syncthreads();
     int at = incl - sum;
-    for (int w = 0; w < warp; ++w) at += warp_sums[w];
+#pragma unroll 4
+    for (int w = 0; w < G::THREADS / 32; ++w) at += w < warp ? warp_sums[w] : 0;
+#pragma unroll 1
     for (int b = b0; b < b1; ++b) {
       prefix[b] = at;
-      at += span_tiles<G::TK>(seq_span(lens[b], p.q_len, p.window));
+      at += span_tiles<G>(seq_span(lens[b], p.q_len, p.window));
     }
     if (tid == G::THREADS - 1) prefix[p.batch] = at;
     __syncthreads();
   }
-  const int per = p.kv_heads * p.n_rb;
+  const int per = p.kv_heads / G::HG * p.n_rb;
   const int total = prefix[p.batch] * per;
-  // at least one tile for each CTA that takes part: no CTA between two that share a unit is
-  // without a part of it
-  const int grid = min(static_cast<int>(gridDim.x), total);
+  // the first `total % gridDim` CTAs take one tile more; some none, behind all others
+  const int share = total / static_cast<int>(gridDim.x), more = total % static_cast<int>(gridDim.x);
+  const int i0 = share * cta + min(cta, more), i1 = i0 + share + (cta < more ? 1 : 0);
 
-  // ---- which CTAs a unit spans; rows of empty sequences
-  for (int u = cta; u < p.batch * per; u += gridDim.x) {
-    const int b = u / per, hb = u - b * per;
-    const int tiles = prefix[b + 1] - prefix[b];
-    if (tiles > 0) {
-      if (tid == 0) {
-        const int first = prefix[b] * per + hb * tiles;
-        p.units[u] = make_int2(share_owner(total, grid, first),
-                               share_owner(total, grid, first + tiles - 1));
+  // ---- the copying warps: all rings, a tile at a time.  Their instructions per tile are what
+  // a small stage would be bound by (one dependent instruction after another)
+  if (warp >= G::W) {
+    if (G::MOVE_REGS) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::REGS_COPY));
+    if (i0 >= i1 || (!p.gather && warp > G::W)) return;
+    Walk<G> ld;
+    ld.start(p, prefix, lens, per, i0);
+    if (p.gather) {
+      // Pages too small for boxes: thread t copies piece t % CPR of every (128 / CPR)-th row,
+      // for all heads of the unit; a page lookup a row.  Arrives at `full` when its copies have.
+      constexpr int CPR = G::DPB / 16, ROWS = kCopyThreads / CPR, PIECES = G::PITCH / 16;
+      const int ct = tid - G::CONSUMERS, c = ct % CPR;
+      const bool in_row = c * 16 < p.dim * G::ELT;
+      int stage = 0;
+      uint32_t parity = 1;
+#pragma unroll 1
+      for (int i = i0; i < i1; ++i) {
+#pragma unroll 1
+        for (int kgr = 0; kgr < G::KG; ++kgr) {
+          if (!mbar_wait(bar_free + kgr * G::MAX_STAGES + stage, parity)) {
+            if (p.status) atomicCAS(p.status, 0, IQ_ERR_PIPE_TIMEOUT);
+            i = i1;
+            break;
+          }
+          const uint32_t to = smem_u32(ring) + (kgr * G::STAGES + stage) * G::STAGE + c / PIECES * G::BOX;
+#pragma unroll 2
+          for (int r = ct / CPR; r < G::KPW; r += ROWS) {
+            const int j = ld.j + kgr * G::KPW + r;
+            int row = -1;
+            if (j >= ld.lo && j < ld.n) {
+              row = cache_row(p.pages, ld.b, j);
+              if (row < 0 && p.status) atomicCAS(p.status, 0, IQ_ERR_ROUTE);
+            }
+            const bool ok = row >= 0 && in_row;  // else zeros, and nothing is read
+            const long long at = ok ? row : 0;
+            const int piece = ok ? c * 16 : 0;
+            const uint8_t* k = p.k + at * p.k_row + ld.h0 * p.k_head + piece;
+            const uint8_t* v = p.v + at * p.v_row + ld.h0 * p.v_head + piece;
+            uint32_t dst = to + swizzled<G>(r, c % PIECES);
+#pragma unroll
+            for (int hd = 0; hd < G::HG; ++hd) {
+              cp_async16(dst, k, ok);
+              cp_async16(dst + G::HALF, v, ok);
+              dst += G::HEAD;
+              k += p.k_head;
+              v += p.v_head;
+            }
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
+                           smem_u32(bar_full + kgr * G::MAX_STAGES + stage))
+                       : "memory");
+        }
+        if (++stage == G::STAGES) {
+          stage = 0;
+          parity ^= 1;
+        }
+        if (i + 1 < i1) ld.next(p, prefix, lens, per);
       }
-      continue;
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      return;
     }
-    if (tid == 0) p.units[u] = make_int2(0, 0);
-    const int h = hb / p.n_rb, r0 = (hb - h * p.n_rb) * G::RB;
-    const int rows = min(G::RB, p.rows_all - r0);
-    for (int i = tid; i < rows * p.dim; i += G::THREADS) {
-      const int r = r0 + i / p.dim, d = i % p.dim;
-      const int tok = r / p.group, head = h * p.group + r % p.group;
+    // A copy is a box of one page: box_rows rows of box_heads heads, of the keys or the values
+    // of one ring.  A lane makes the same copy of every tile, and has its page read one tile
+    // ahead.
+    const int boxes = G::KPW / p.box_rows, groups = G::HG / p.box_heads;
+    const int copies = 2 * G::BOXES * boxes * groups * G::KG;
+    const int x = (lane >> 1) % G::BOXES, r = (lane >> 1) / G::BOXES, box = r % boxes;
+    const int head = r / boxes % groups * p.box_heads, kgr = r / boxes / groups;
+    const int key = kgr * G::KPW + box * p.box_rows;
+    const uint32_t dst = smem_u32(ring) + kgr * G::STAGES * G::STAGE + (lane & 1) * G::HALF +
+                         x * G::BOX + head * G::HEAD + box * p.box_rows * G::PITCH;
+    auto look_up = [&]() -> int {                // -1 where the box holds no key of the unit
+      const int j = ld.j + key;
+      return j < ld.n && j + p.box_rows > ld.lo ? page_id(p.pages, ld.b, j) : -1;
+    };
+    const CUtensorMap* map = lane & 1 ? &p.v_map : &p.k_map;
+    int id_next = lane < copies ? look_up() : -1, stage = 0;
+    uint32_t parity = 1;
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) {
+      bool ok = true;
+      if (lane < G::KG) {
+        ok = mbar_wait(bar_free + lane * G::MAX_STAGES + stage, parity);
+        if (ok) mbar_arrive_expect_tx(bar_full + lane * G::MAX_STAGES + stage, G::STAGE);
+      }
+      if (!__all_sync(0xffffffffu, ok)) {        // the consumers gave up, or are stuck
+        if (lane == 0 && p.status) atomicCAS(p.status, 0, IQ_ERR_PIPE_TIMEOUT);
+        break;
+      }
+      if (lane < copies) {
+        // a box without keys of the unit, or of a page outside the cache, is read past the
+        // cache's end, which fills it with zeros
+        const int j = ld.j + key;
+        int at = p.pages.capacity;
+        if (j < ld.n && j + p.box_rows > ld.lo) {
+          const int row = page_row(p.pages, id_next, j);
+          if (row >= 0) at = row;
+          else if (p.status) atomicCAS(p.status, 0, IQ_ERR_ROUTE);
+        }
+        tma_3d_g2s(dst + stage * G::STAGE, map, x * G::PITCH, at, ld.h0 + head,
+                   bar_full + kgr * G::MAX_STAGES + stage);
+      }
+      if (++stage == G::STAGES) {
+        stage = 0;
+        parity ^= 1;
+      }
+      if (i + 1 < i1) {
+        ld.next(p, prefix, lens, per);
+        if (lane < copies) id_next = look_up();
+      }
+    }
+    // shared memory must outlive the copies: the last of each stage
+    if (lane < G::KG)
+      for (int s = 0; s < min(G::STAGES, i1 - i0); ++s) {
+        const int rounds = (i1 - i0 - 1 - s) / G::STAGES;   // of this stage before its last
+        mbar_wait(bar_full + lane * G::MAX_STAGES + s, rounds & 1);
+      }
+    return;
+  }
+
+  if (G::MOVE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::REGS_COMPUTE));
+
+  auto sync_all = [&]() { named_bar_sync(1, G::CONSUMERS); };
+  constexpr int GT = 32 * G::WR;
+  const int gtid = wr * 32 + lane;
+  const uint32_t ring_g = smem_u32(ring) + kg * G::STAGES * G::STAGE + hg * G::HEAD;
+  uint64_t* full = bar_full + kg * G::MAX_STAGES;
+  uint64_t* free_ = bar_free + kg * G::MAX_STAGES;
+
+  // ---- rows of empty sequences
+#pragma unroll 1
+  for (int b = cta; b < p.batch; b += gridDim.x) {
+    if (prefix[b + 1] != prefix[b]) continue;
+    for (int u = tid; u < per; u += G::CONSUMERS) p.units[b * per + u] = make_int2(0, 0);
+    for (int i = tid; i < p.q_len * p.q_heads * p.dim; i += G::CONSUMERS) {
+      const int d = i % p.dim, head = i / p.dim % p.q_heads, tok = i / p.dim / p.q_heads;
       p.out[b * p.o_b + tok * p.o_r + head * p.o_h + d] = __float2bfloat16_rn(0.f);
       if (d == 0) {
         const long long o = (static_cast<long long>(b) * p.q_len + tok) * p.q_heads + head;
@@ -296,107 +555,66 @@ __global__ void __launch_bounds__(G::THREADS, G::CTAS) attn_kernel(const __grid_
       }
     }
   }
-
-  if (cta >= grid) return;
-  const int i0 = share_begin(total, grid, cta), i1 = share_begin(total, grid, cta + 1);
-
-  // ---- copies: this warp's part of its key group's ring
-  const uint32_t ring_g = smem_u32(ring) + kg * G::STAGES * G::STAGE;
-  constexpr int GT = 32 * G::WR;
-  const int gtid = wr * 32 + lane;
-  TileIter ld;
-  iter_init<G>(ld, p, prefix, lens, i0);
-  auto look_up = [&]() -> int {                  // lanes 0..15: the cache row of key `lane`
-    const int j = ld.s.lo + ld.tile * G::TK + kg * 16 + lane;
-    if (lane >= 16 || j >= ld.s.hi) return -1;
-    const int row = cache_row(p.pages, ld.b, j);
-    if (row < 0 && p.status) atomicCAS(p.status, 0, IQ_ERR_ROUTE);
-    return row;
-  };
-  int row_next = look_up();
-  auto issue = [&](int stage) {
-    const int h = ld.hb / p.n_rb;
-    const uint32_t dst_k = ring_g + stage * G::STAGE, dst_v = dst_k + 16 * G::DPB;
-#pragma unroll
-    for (int i = 0; i < (16 * G::CPR + GT - 1) / GT; ++i) {
-      const int idx = gtid + i * GT;
-      const int r = idx / G::CPR, c = idx % G::CPR;
-      const int row = __shfl_sync(0xffffffffu, row_next, r & 15);
-      if (16 * G::CPR % GT == 0 || idx < 16 * G::CPR) {
-        const bool ok = row >= 0 && c * 16 < p.dim * G::ELT;
-        const long long rr = ok ? row : 0;
-        const int cc = ok ? c * 16 : 0;
-        int ck, cv;
-        if (G::KV == IQ_ACT_BF16) {
-          ck = cv = c ^ (r & 7);
-        } else {
-          ck = G::DPB >= 128 ? c ^ ((r & 1) << 2) : c;
-          cv = G::DPB >= 128 ? c ^ (((r >> 1) & 3) << 1) : c ^ ((r >> 1) & 3);
-        }
-        cp_async16(dst_k + r * G::DPB + ck * 16, p.k + rr * p.k_row + h * p.k_head + cc, ok);
-        cp_async16(dst_v + r * G::DPB + cv * 16, p.v + rr * p.v_row + h * p.v_head + cc, ok);
-      }
-    }
-  };
-  int ld_at = i0;
-  auto feed = [&](int stage) {                   // the next tile's copies, and one group always
-    if (ld_at < i1) {
-      issue(stage);
-      if (++ld_at < i1) {
-        iter_next<G>(ld, p, prefix, lens);
-        row_next = look_up();
-      }
-    }
-    cp_async_commit();
-  };
-  auto group_sync = [&]() {
-    if (G::WR == 1) __syncwarp();
-    else if (G::WK == 1) __syncthreads();
-    else named_bar_sync(1 + kg, GT);
-  };
-
-#pragma unroll
-  for (int s = 0; s < G::STAGES - 1; ++s) feed(s);
+  if (i0 >= i1) return;
+  Walk<G> it;
+  bool from_start = it.start(p, prefix, lens, per, i0) == 0;   // the segment begins where its unit begins
 
   // ---- state of the unit being computed
-  constexpr int QREG = G::DP / 8;                // packed registers of q a block of eight rows
-  uint32_t qf[G::NBW][QREG];
+  uint32_t qf[G::QS ? 1 : G::NBW][G::QREG];
+  uint32_t* q_mine = q_smem + ((hg * G::WR + wr) * G::NBW) * G::QREG * 32 + 2 * lane;   // [nb][reg / 2][lane][2]
   float xs[G::NBW][2];                           // score factor of this lane's two columns
-  float m[G::NBW][2], l[G::NBW][2], acc[G::NBW][G::MT][4];
-  bool have_edges = false;
+  // m: the reference the weights are relative to; mu: the same, 0 while there is none; thr:
+  // how far above it a score may lie before the reference moves
+  float m[G::NBW][2], mu[G::NBW][2], thr[G::NBW][2], l[G::NBW][2], acc[G::NBW][G::MT][4];
 
-  // P relative to 2^14 in half precision (e4m3 caches): the weights that a fixed-point
-  // format would lose lie fourteen bits lower; bf16 has fp32's range and needs no shift.
-  constexpr float kShift = G::KV == IQ_ACT_BF16 ? 0.f : 14.f;
+  // The reference only has to keep the weights inside their type's range, so it follows the
+  // maximum lazily: it moves when a score lies more than kLimit above it, to kShift below
+  // that score.  Half precision (e4m3 caches): weights up to 2^15; what is 2^-22 of the
+  // largest starts to lose bits.  bf16 has fp32's range.
+  constexpr float kShift = G::KV == IQ_ACT_BF16 ? 0.f : 8.f;
+  constexpr float kLimit = G::KV == IQ_ACT_BF16 ? 8.f : 15.f;
+  const int key_lo = key_of<G>(g);               // this lane's keys of a tile of 16: key_lo, + 8
+  // Where this lane's fragment loads of a tile start; the others lie at fixed distances, or
+  // (other pieces of a swizzled row) at the address with a constant xored in.  bf16: ldmatrix
+  // of the keys (matrices: keys 0-7, 8-15, then their next eight channels) and transposed of
+  // the values (channels 0-7, 8-15 of keys 0-7, then of keys 8-15).  e4m3: 16 bytes (values at
+  // D = 64: 8) of a row a load.
+  uint32_t k_lane, v_lane, v_odd = 0;
+  if (G::KV == IQ_ACT_BF16) {
+    k_lane = ring_g + swizzled<G>(lane & 15, lane >> 4);
+    v_lane = ring_g + G::HALF + swizzled<G>((lane & 7) + (lane >> 4) * 8, lane >> 3 & 1);
+  } else {
+    k_lane = ring_g + swizzled<G>(key_lo, t);
+    const int c = G::DP >= 128 ? g : g >> 1, in = G::DP >= 128 ? 0 : (g & 1) * 8;
+    v_lane = ring_g + G::HALF + swizzled<G>(key_of<G>(2 * t), c) + in;
+    v_odd = swizzled<G>(key_of<G>(2 * t + 1), c) - swizzled<G>(key_of<G>(2 * t), c);
+  }
 
-  TileIter it;
-  iter_init<G>(it, p, prefix, lens, i0);
-  bool fresh = true;
-  int seg_first_tile = it.tile;                  // place of the segment's first tile in its unit
+  bool fresh = true, dead = false;
+  int seg_key = 0;                               // the segment's first key
+  int slot = 0;
+  uint32_t parity = 0;
 
+#pragma unroll 1
   for (int i = i0; i < i1; ++i) {
-    const int slot = (i - i0) % G::STAGES;
-    cp_async_wait<G::STAGES - 2>();
-    group_sync();
-    feed((i - i0 + G::STAGES - 1) % G::STAGES);
-
-    const int h = it.hb / p.n_rb, r0 = (it.hb - h * p.n_rb) * G::RB;
+    const int h = it.h0 + hg, r0 = it.r0;
     if (fresh) {
       fresh = false;
-      have_edges = false;
-      seg_first_tile = it.tile;
+      seg_key = it.j;
+      if (from_start && tid == 0) p.units[it.b * per + it.hb].x = cta;
 #pragma unroll
       for (int nb = 0; nb < G::NBW; ++nb) {
         const int r = r0 + (wr * G::NBW + nb) * 8 + g;
         const bool live = r < p.rows_all;
-        const int tok = live ? r / p.group : 0, head = h * p.group + (live ? r % p.group : 0);
+        const int tok = live ? r / p.group : 0, head = h * p.group + (live ? r - tok * p.group : 0);
         const __nv_bfloat16* src = p.q + it.b * p.q_b + tok * p.q_r + head * p.q_h;
+        uint32_t(&qr)[G::QREG] = qf[G::QS ? 0 : nb];
         if (G::KV == IQ_ACT_BF16) {
           // fragment order of the MMA: registers 2i, 2i+1 are channels 16i + 2t, 16i + 8 + 2t
 #pragma unroll
-          for (int x = 0; x < QREG; ++x) {
+          for (int x = 0; x < G::QREG; ++x) {
             const int d = x * 8 + 2 * t;
-            qf[nb][x] = live && d < p.dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+            qr[x] = live && d < p.dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
           }
           xs[nb][0] = xs[nb][1] = p.scale_log2;
         } else {
@@ -405,13 +623,16 @@ __global__ void __launch_bounds__(G::THREADS, G::CTAS) attn_kernel(const __grid_
           // values 2^-14 below the row's largest
           float big = 0.f;
 #pragma unroll
-          for (int x = 0; x < QREG; ++x) {
+          for (int x = 0; x < G::QREG; x += 4) {
             const int d = (x / 8) * 64 + t * 16 + (x % 8) * 2;
-            const uint32_t w = live && d < p.dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
-            qf[nb][x] = w;
-            big = fmaxf(big, fmaxf(fabsf(__uint_as_float(w << 16)),
-                                   fabsf(__uint_as_float(w & 0xffff0000u))));
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (live && d < p.dim) w = *reinterpret_cast<const uint4*>(src + d);
+            qr[x] = w.x; qr[x + 1] = w.y; qr[x + 2] = w.z; qr[x + 3] = w.w;
           }
+#pragma unroll
+          for (int x = 0; x < G::QREG; ++x)
+            big = fmaxf(big, fmaxf(fabsf(__uint_as_float(qr[x] << 16)),
+                                   fabsf(__uint_as_float(qr[x] & 0xffff0000u))));
           big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
           big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
           int e = static_cast<int>(__float_as_uint(big) >> 23) - 127;
@@ -420,440 +641,553 @@ __global__ void __launch_bounds__(G::THREADS, G::CTAS) attn_kernel(const __grid_
           const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
           const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 #pragma unroll
-          for (int x = 0; x < QREG; ++x) {
-            const uint32_t w = qf[nb][x];
-            qf[nb][x] = pack_f16(__uint_as_float(w << 16) * down,
-                                 __uint_as_float(w & 0xffff0000u) * down);
-          }
+          for (int x = 0; x < G::QREG; ++x)
+            qr[x] = pack_f16(__uint_as_float(qr[x] << 16) * down,
+                             __uint_as_float(qr[x] & 0xffff0000u) * down);
           const float f = p.scale_log2 * up;
           xs[nb][0] = __shfl_sync(0xffffffffu, f, (2 * t) * 4);
           xs[nb][1] = __shfl_sync(0xffffffffu, f, (2 * t + 1) * 4);
         }
-        m[nb][0] = m[nb][1] = -INFINITY;
-        l[nb][0] = l[nb][1] = 0.f;
+        if (G::QS && kg == 0)
+#pragma unroll
+          for (int x = 0; x < G::QREG; x += 2)
+            *reinterpret_cast<uint2*>(q_mine + (nb * G::QREG + x) * 32) = make_uint2(qr[x], qr[x + 1]);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          m[nb][c] = -INFINITY;
+          mu[nb][c] = 0.f;
+          thr[nb][c] = -INFINITY;
+          l[nb][c] = 0.f;
+        }
 #pragma unroll
         for (int x = 0; x < G::MT; ++x)
           acc[nb][x][0] = acc[nb][x][1] = acc[nb][x][2] = acc[nb][x][3] = 0.f;
       }
+      if (G::QS) sync_all();
     }
 
-    const int common = (it.s.hi - it.s.lo + G::TK - 1) / G::TK;
-    const int j0 = it.s.lo + it.tile * G::TK + kg * 16;
-    if (it.tile < common && j0 < it.s.hi) {
-      const uint32_t sk = ring_g + slot * G::STAGE, sv = sk + 16 * G::DPB;
-      float sc[G::NBW][4];
+    const int j0 = it.j + kg * G::KPW;
+    // some key of these is not seen by every row
+    const int lo_all = p.window ? max(0, it.n - p.window) : 0, hi_all = max(it.n - p.q_len + 1, 0);
+    const bool partial = j0 < lo_all || j0 + G::KPW > hi_all;
+    const uint32_t sv = ring_g + slot * G::STAGE + G::HALF;
+    if (!dead && __any_sync(0xffffffffu, !mbar_wait(full + slot, parity))) {
+      dead = true;                               // (the whole warp: it waits no more)
+      if (lane == 0 && p.status) atomicCAS(p.status, 0, IQ_ERR_PIPE_TIMEOUT);
+    }
+    if (partial) {
+      // values outside the unit: zeros; values that only some rows see: finite ones stay
+#pragma unroll 1
+      for (int x = gtid; x < G::KPW * G::DPB / 16; x += GT) {
+        const int j = j0 + (x / (G::PITCH / 16)) % G::KPW;
+        if (j >= lo_all && j < hi_all) continue;
+        const uint32_t at = sv + x / (G::HEAD / 16) * G::BOX + x % (G::HEAD / 16) * 16;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (j >= it.lo && j < it.n) {
+          w = lds128(at);
+          if (!strip<G::KV>(w)) continue;
+          *not_finite = 1;
+        }
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w.x),
+                     "r"(w.y), "r"(w.z), "r"(w.w)
+                     : "memory");
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (G::WR == 1) __syncwarp();
+      else named_bar_sync(2 + warp / G::WR, GT);
+    }
+
+    // The tiles of sixteen keys, SUBI at a time.  EDGE: some row does not see some key, or the
+    // scores are kept; the other form, nearly all tiles', has no branch but the reference's.
+    auto tiles = [&](auto edge) {
+      constexpr bool EDGE = decltype(edge)::value;
+#pragma unroll 1
+      for (int s0 = 0; s0 < G::SUB; s0 += G::SUBI) {
+        if (EDGE && (j0 + s0 * 16 >= it.n || j0 + (s0 + G::SUBI) * 16 <= it.lo)) continue;
+        const uint32_t tk = k_lane + slot * G::STAGE + s0 * 16 * G::PITCH;
+        const uint32_t tv = v_lane + slot * G::STAGE + s0 * 16 * G::PITCH;
+        float sc[G::SUBI][G::NBW][4];
 #pragma unroll
-      for (int nb = 0; nb < G::NBW; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
-      if (G::KV == IQ_ACT_BF16) {
-        const int r = (lane & 7) + ((lane >> 3) & 1) * 8;       // matrices: keys 0-7, 8-15
-#pragma unroll
-        for (int x = 0; x < G::MT; ++x) {
-          uint32_t a[4];
-          ldmatrix_x4(a, sk + r * G::DPB + (((2 * x + (lane >> 4)) ^ (r & 7)) * 16));
+        for (int sub = 0; sub < G::SUBI; ++sub)
 #pragma unroll
           for (int nb = 0; nb < G::NBW; ++nb)
-            mma_bf16(sc[nb], a[0], a[1], a[2], a[3], qf[nb][2 * x], qf[nb][2 * x + 1]);
-        }
-      } else {
-#pragma unroll
-        for (int kk = 0; kk < G::DP / 64; ++kk) {
-          const int c = G::DPB >= 128 ? (kk * 4 + t) ^ ((g & 1) << 2) : kk * 4 + t;
-          const uint4 lo = lds128(sk + g * G::DPB + c * 16);
-          const uint4 hi = lds128(sk + (g + 8) * G::DPB + c * 16);
-          const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint32_t a0 = e4m3x2_to_f16x2(wl[x]), a2 = e4m3x2_to_f16x2(wl[x] >> 16);
-            const uint32_t a1 = e4m3x2_to_f16x2(wh[x]), a3 = e4m3x2_to_f16x2(wh[x] >> 16);
-#pragma unroll
-            for (int nb = 0; nb < G::NBW; ++nb)
-              mma_f16(sc[nb], a0, a1, a2, a3, qf[nb][kk * 8 + 2 * x], qf[nb][kk * 8 + 2 * x + 1]);
-          }
-        }
-      }
-      // ---- softmax of this lane's columns (query rows 2t, 2t+1), keys g and g + 8
-      uint32_t pb[G::NBW][2];
-      const bool lo_ok = j0 + g < it.s.hi, hi_ok = j0 + g + 8 < it.s.hi;
-#pragma unroll
-      for (int nb = 0; nb < G::NBW; ++nb) {
-        float x0 = sc[nb][0] * xs[nb][0], x1 = sc[nb][1] * xs[nb][1];
-        float x2 = sc[nb][2] * xs[nb][0], x3 = sc[nb][3] * xs[nb][1];
-        if (p.scores) {
-          const int r = r0 + (wr * G::NBW + nb) * 8 + 2 * t;
-          if (r < p.rows_pad) {
-            float* dst = p.scores +
-                         ((static_cast<long long>(it.b) * p.kv_heads + h) * p.score_rows + j0 + g) *
-                             p.rows_pad + r;
-            if (lo_ok) *reinterpret_cast<float2*>(dst) = make_float2(x0, x1);
-            if (hi_ok) *reinterpret_cast<float2*>(dst + 8 * p.rows_pad) = make_float2(x2, x3);
-          }
-        }
-        if (!lo_ok) x0 = x1 = -INFINITY;
-        if (!hi_ok) x2 = x3 = -INFINITY;
-        float t0 = fmaxf(x0, x2), t1 = fmaxf(x1, x3);
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, o));
-          t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, o));
-        }
-        t0 = fmaxf(t0 - kShift, m[nb][0]);
-        t1 = fmaxf(t1 - kShift, m[nb][1]);
-        const float u0 = t0 == -INFINITY ? 0.f : t0, u1 = t1 == -INFINITY ? 0.f : t1;
-        const bool moved = t0 != m[nb][0] || t1 != m[nb][1];
-        if (__any_sync(0xffffffffu, moved)) {
-          const float c0 = ex2(m[nb][0] - u0), c1 = ex2(m[nb][1] - u1);
-          l[nb][0] *= c0;
-          l[nb][1] *= c1;
+            sc[sub][nb][0] = sc[sub][nb][1] = sc[sub][nb][2] = sc[sub][nb][3] = 0.f;
+        // ---- S^T = K Q^T (the tiles interleaved: independent sums)
+        auto q_frag = [&](int nb, int x) {       // registers 2x, 2x + 1
+          if (!G::QS) return make_uint2(qf[nb][2 * x], qf[nb][2 * x + 1]);
+          return lds64(smem_u32(q_mine + (nb * G::QREG + 2 * x) * 32));
+        };
+        if (G::KV == IQ_ACT_BF16) {
 #pragma unroll
           for (int x = 0; x < G::MT; ++x) {
-            acc[nb][x][0] *= c0;
-            acc[nb][x][1] *= c1;
-            acc[nb][x][2] *= c0;
-            acc[nb][x][3] *= c1;
-          }
-          m[nb][0] = t0;
-          m[nb][1] = t1;
-        }
-        x0 = ex2(x0 - u0);
-        x1 = ex2(x1 - u1);
-        x2 = ex2(x2 - u0);
-        x3 = ex2(x3 - u1);
-        // the normaliser adds the weights as computed; the products below take them rounded
-        // to the MMA's type (half: 2^-11, bf16: 2^-8 relative at most, of random sign)
-        l[nb][0] += x0 + x2;
-        l[nb][1] += x1 + x3;
-        if (G::KV == IQ_ACT_BF16) {
-          pb[nb][0] = transpose8x8(pack_bf16(x0, x1));
-          pb[nb][1] = transpose8x8(pack_bf16(x2, x3));
-        } else {
-          pb[nb][0] = transpose8x8(pack_f16(x0, x1));
-          pb[nb][1] = transpose8x8(pack_f16(x2, x3));
-        }
-      }
-      // ---- O^T += V^T P^T
-      if (G::KV == IQ_ACT_BF16) {
-        const int r = (lane & 7) + (lane >> 4) * 8;             // matrices: d 0-7, d 8-15 of keys 0-7; of keys 8-15
+            uint2 b[G::NBW];
 #pragma unroll
-        for (int x = 0; x < G::MT; ++x) {
-          uint32_t a[4];
-          ldmatrix_x4_trans(a, sv + r * G::DPB + (((2 * x + ((lane >> 3) & 1)) ^ (r & 7)) * 16));
+            for (int nb = 0; nb < G::NBW; ++nb) b[nb] = q_frag(nb, x);
 #pragma unroll
-          for (int nb = 0; nb < G::NBW; ++nb)
-            mma_bf16(acc[nb][x], a[0], a[1], a[2], a[3], pb[nb][0], pb[nb][1]);
-        }
-      } else {
-        // lane g holds channels 128 dd + 16 g .. + 15 (8 g .. + 7 for D = 64) of the keys
-        // 2t, 2t+1, 2t+8, 2t+9; pairs of keys are interleaved bytewise, then widened
-        constexpr int WORDS = G::DP >= 128 ? 4 : 2;
-#pragma unroll
-        for (int dd = 0; dd < (G::DP + 127) / 128; ++dd) {
-          uint32_t v[4][WORDS];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const int r = 2 * t + (y & 1) + (y >> 1) * 8;
-            if (G::DP >= 128) {
-              const uint4 w = lds128(sv + r * G::DPB + (((dd * 8 + g) ^ (((r >> 1) & 3) << 1)) * 16));
-              v[y][0] = w.x; v[y][1] = w.y; v[y][WORDS - 2] = w.z; v[y][WORDS - 1] = w.w;
-            } else {
-              const uint2 w = lds64(sv + r * G::DPB + (((g >> 1) ^ ((r >> 1) & 3)) * 16) + (g & 1) * 8);
-              v[y][0] = w.x; v[y][1] = w.y;
-            }
-          }
-#pragma unroll
-          for (int w = 0; w < WORDS; ++w) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint32_t p01 = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140);
-              const uint32_t p89 = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
-              const uint32_t a0 = e4m3x2_to_f16x2(p01), a1 = e4m3x2_to_f16x2(p01 >> 16);
-              const uint32_t a2 = e4m3x2_to_f16x2(p89), a3 = e4m3x2_to_f16x2(p89 >> 16);
-              const int x = dd * 8 + 2 * w + half;
+            for (int sub = 0; sub < G::SUBI; ++sub) {
+              uint32_t a[4];
+              ldmatrix_x4(a, (tk ^ (x % 4 * 32)) + x / 4 * G::BOX + sub * 16 * G::PITCH);
 #pragma unroll
               for (int nb = 0; nb < G::NBW; ++nb)
-                mma_f16(acc[nb][x], a0, a1, a2, a3, pb[nb][0], pb[nb][1]);
+                mma_k16<G::KV>(sc[sub][nb], a[0], a[1], a[2], a[3], b[nb].x, b[nb].y);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int kk = 0; kk < G::DP / 64; ++kk) {
+            const uint32_t box = (tk ^ (kk % 2 * 64)) + kk / 2 * G::BOX;
+            uint32_t wl[G::SUBI][4], wh[G::SUBI][4];
+#pragma unroll
+            for (int sub = 0; sub < G::SUBI; ++sub) {
+              const uint4 lo = lds128(box + sub * 16 * G::PITCH);
+              const uint4 hi = lds128(box + (sub * 16 + 8) * G::PITCH);
+              wl[sub][0] = lo.x; wl[sub][1] = lo.y; wl[sub][2] = lo.z; wl[sub][3] = lo.w;
+              wh[sub][0] = hi.x; wh[sub][1] = hi.y; wh[sub][2] = hi.z; wh[sub][3] = hi.w;
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              uint2 b[G::NBW];
+#pragma unroll
+              for (int nb = 0; nb < G::NBW; ++nb) b[nb] = q_frag(nb, kk * 4 + x);
+#pragma unroll
+              for (int sub = 0; sub < G::SUBI; ++sub) {
+                const uint32_t a0 = e4m3x2_to_f16x2(wl[sub][x]), a2 = e4m3x2_to_f16x2(wl[sub][x] >> 16);
+                const uint32_t a1 = e4m3x2_to_f16x2(wh[sub][x]), a3 = e4m3x2_to_f16x2(wh[sub][x] >> 16);
+#pragma unroll
+                for (int nb = 0; nb < G::NBW; ++nb)
+                  mma_k16<G::KV>(sc[sub][nb], a0, a1, a2, a3, b[nb].x, b[nb].y);
+              }
+            }
+          }
+        }
+        // ---- softmax of this lane's columns (query rows 2t, 2t+1) and two keys a tile
+        const int jt = j0 + s0 * 16 + key_lo;
+        float x[G::NBW][G::SUBI][4];
+        auto masked = [&](int nb) {              // -infinity for what this lane's rows do not see
+          if (!EDGE) return;
+          const int r = r0 + (wr * G::NBW + nb) * 8 + 2 * t;
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int pos = it.n - p.q_len + min((r + y) / p.group, p.q_len - 1);
+            const int from = p.window ? max(0, pos - p.window + 1) : 0;
+#pragma unroll
+            for (int sub = 0; sub < G::SUBI; ++sub)
+#pragma unroll
+              for (int z = 0; z < 2; ++z) {
+                const int key = jt + sub * 16 + z * 8;
+                if (key < from || key > pos) x[nb][sub][2 * z + y] = -INFINITY;
+              }
+          }
+        };
+        if (EDGE && p.scores) {
+#pragma unroll
+          for (int nb = 0; nb < G::NBW; ++nb) {
+            const int r = r0 + (wr * G::NBW + nb) * 8 + 2 * t;
+            if (r >= p.rows_pad) continue;
+#pragma unroll
+            for (int sub = 0; sub < G::SUBI; ++sub)
+#pragma unroll
+              for (int y = 0; y < 4; ++y) x[nb][sub][y] = sc[sub][nb][y] * xs[nb][y & 1];
+            if (partial) masked(nb);
+#pragma unroll
+            for (int sub = 0; sub < G::SUBI; ++sub) {
+              const int j = jt + sub * 16;
+              float* dst = p.scores +
+                           ((static_cast<long long>(it.b) * p.kv_heads + h) * p.score_rows + j) *
+                               p.rows_pad + r;
+              const float(&z)[4] = x[nb][sub];
+              if (j >= it.lo && j < it.n) *reinterpret_cast<float2*>(dst) = make_float2(z[0], z[1]);
+              if (j + 8 >= it.lo && j + 8 < it.n)
+                *reinterpret_cast<float2*>(dst + 8 * p.rows_pad) = make_float2(z[2], z[3]);
+            }
+          }
+        }
+        float top[G::NBW][2];
+        bool above = false;
+        auto shifted = [&](int nb) {
+#pragma unroll
+          for (int sub = 0; sub < G::SUBI; ++sub)
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              x[nb][sub][y] = fmaf(sc[sub][nb][y], xs[nb][y & 1], -mu[nb][y & 1]);
+          if (EDGE && partial) masked(nb);
+        };
+#pragma unroll
+        for (int nb = 0; nb < G::NBW; ++nb) {
+          shifted(nb);
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            top[nb][y] = fmaxf(x[nb][0][y], x[nb][0][y + 2]);
+#pragma unroll
+            for (int sub = 1; sub < G::SUBI; ++sub)
+              top[nb][y] = fmaxf(top[nb][y], fmaxf(x[nb][sub][y], x[nb][sub][y + 2]));
+            above |= top[nb][y] > thr[nb][y];
+          }
+        }
+        if (__any_sync(0xffffffffu, above)) {    // the references move
+#pragma unroll
+          for (int nb = 0; nb < G::NBW; ++nb) {
+            float c[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              float best = top[nb][y] + mu[nb][y];
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+              best = fmaxf(best - kShift, m[nb][y]);
+              const float u = best == -INFINITY ? 0.f : best;
+              c[y] = ex2(m[nb][y] - u);
+              m[nb][y] = best;
+              mu[nb][y] = u;
+              thr[nb][y] = best == -INFINITY ? -INFINITY : kLimit;
+              l[nb][y] *= c[y];
+            }
+#pragma unroll
+            for (int y = 0; y < G::MT; ++y) {
+              acc[nb][y][0] *= c[0];
+              acc[nb][y][1] *= c[1];
+              acc[nb][y][2] *= c[0];
+              acc[nb][y][3] *= c[1];
+            }
+            shifted(nb);
+          }
+        }
+        uint32_t pb[G::SUBI][G::NBW][2];
+#pragma unroll
+        for (int sub = 0; sub < G::SUBI; ++sub) {
+#pragma unroll
+          for (int nb = 0; nb < G::NBW; ++nb) {
+            float(&z)[4] = x[nb][sub];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) z[y] = ex2(z[y]);
+            // the normaliser adds the weights as computed; the products below take them
+            // rounded to the MMA's type (half: 2^-11, bf16: 2^-8 relative at most)
+            l[nb][0] += z[0] + z[2];
+            l[nb][1] += z[1] + z[3];
+            if (G::KV == IQ_ACT_BF16) {
+              pb[sub][nb][0] = transpose8x8(pack_bf16(z[0], z[1]));
+              pb[sub][nb][1] = transpose8x8(pack_bf16(z[2], z[3]));
+            } else {
+              pb[sub][nb][0] = transpose8x8(pack_f16(z[0], z[1]));
+              pb[sub][nb][1] = transpose8x8(pack_f16(z[2], z[3]));
+            }
+          }
+        }
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int sub = 0; sub < G::SUBI; ++sub) {
+          if (G::KV == IQ_ACT_BF16) {
+#pragma unroll
+            for (int x_ = 0; x_ < G::MT; ++x_) {
+              uint32_t a[4];
+              ldmatrix_x4_trans(a, (tv ^ (x_ % 4 * 32)) + x_ / 4 * G::BOX + sub * 16 * G::PITCH);
+#pragma unroll
+              for (int nb = 0; nb < G::NBW; ++nb)
+                mma_k16<G::KV>(acc[nb][x_], a[0], a[1], a[2], a[3], pb[sub][nb][0], pb[sub][nb][1]);
+            }
+          } else {
+            // lane g holds channels 128 dd + 16 g .. + 15 (8 g .. + 7 for D = 64) of the keys
+            // in rows 2t, 2t+1, 2t+8, 2t+9; pairs of keys are interleaved bytewise, then widened
+            constexpr int WORDS = G::DP >= 128 ? 4 : 2;
+#pragma unroll
+            for (int dd = 0; dd < (G::DP + 127) / 128; ++dd) {
+              uint32_t v[4][WORDS];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                const uint32_t at = (y & 1 ? tv + v_odd : tv) + dd * G::BOX + (sub * 16 + (y >> 1) * 8) * G::PITCH;
+                if (G::DP >= 128) {
+                  const uint4 w = lds128(at);
+                  v[y][0] = w.x; v[y][1] = w.y; v[y][WORDS - 2] = w.z; v[y][WORDS - 1] = w.w;
+                } else {
+                  const uint2 w = lds64(at);
+                  v[y][0] = w.x; v[y][1] = w.y;
+                }
+              }
+#pragma unroll
+              for (int w = 0; w < WORDS; ++w) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  const uint32_t p01 = __byte_perm(v[0][w], v[1][w], half ? 0x7362 : 0x5140);
+                  const uint32_t p89 = __byte_perm(v[2][w], v[3][w], half ? 0x7362 : 0x5140);
+                  const uint32_t a0 = e4m3x2_to_f16x2(p01), a1 = e4m3x2_to_f16x2(p01 >> 16);
+                  const uint32_t a2 = e4m3x2_to_f16x2(p89), a3 = e4m3x2_to_f16x2(p89 >> 16);
+                  const int x_ = dd * 8 + 2 * w + half;
+#pragma unroll
+                  for (int nb = 0; nb < G::NBW; ++nb)
+                    mma_k16<G::KV>(acc[nb][x_], a0, a1, a2, a3, pb[sub][nb][0], pb[sub][nb][1]);
+                }
+              }
             }
           }
         }
       }
+    };
+    if (!partial && !p.scores) tiles(std::false_type{});
+    else if (j0 < it.n && j0 + G::KPW > it.lo) tiles(std::true_type{});
+
+    // the stage is free: one arrival a warp that reads it
+    __syncwarp();
+    if (lane == 0) mbar_arrive(free_ + slot);
+    if (++slot == G::STAGES) {
+      slot = 0;
+      parity ^= 1;
     }
 
-    const bool edge_tile = it.tile >= common;
-    const bool unit_end = it.tile == it.tiles - 1;
+    const bool unit_end = it.left == 1;
     if (unit_end || i == i1 - 1) {
       // ---- the unit ends here, or the share does: join the warps' keys
 #pragma unroll
-      for (int nb = 0; nb < G::NBW; ++nb)
+      for (int nb = 0; nb < G::NBW; ++nb) {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], o);
-#pragma unroll
-      for (int nb = 0; nb < G::NBW; ++nb) {
 #pragma unroll 1
-        for (int half = G::WK / 2; half >= 1; half >>= 1) {
-          float* mine = join + (((kg & (half - 1)) * G::WR + wr) * G::NREG) * 32 + lane;
-          if (kg >= half && kg < 2 * half) {
+        for (int half = G::KG / 2; half >= 1; half >>= 1) {
+          float* mine = join + ((((kg & (half - 1)) * G::HG + hg) * G::WR + wr) * G::NREG) * 32 + 4 * lane;
+          constexpr int MX = G::MT / G::XP;
+          float f[2], e[2];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              mine[64 * c] = m[nb][c];
-              mine[64 * c + 32] = l[nb][c];
-            }
+          for (int part = 0; part < G::XP; ++part) {
+            if (kg >= half && kg < 2 * half) {
+              if (part == 0)
+                *reinterpret_cast<float4*>(mine) = make_float4(m[nb][0], m[nb][1], l[nb][0], l[nb][1]);
 #pragma unroll
-            for (int x = 0; x < G::MT; ++x)
-#pragma unroll
-              for (int y = 0; y < 4; ++y) mine[32 * (4 + 4 * x + y)] = acc[nb][x][y];
-          }
-          __syncthreads();
-          if (kg < half) {
-            float f[2], e[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const float om = mine[64 * c], ol = mine[64 * c + 32];
-              const float top = fmaxf(m[nb][c], om), u = top == -INFINITY ? 0.f : top;
-              f[c] = ex2(m[nb][c] - u);
-              e[c] = ex2(om - u);
-              m[nb][c] = top;
-              l[nb][c] = l[nb][c] * f[c] + ol * e[c];
-            }
-#pragma unroll
-            for (int x = 0; x < G::MT; ++x)
-#pragma unroll
-              for (int y = 0; y < 4; ++y)
-                acc[nb][x][y] = acc[nb][x][y] * f[y & 1] + mine[32 * (4 + 4 * x + y)] * e[y & 1];
-          }
-          __syncthreads();
-        }
-      }
-      // ---- the edge keys, row by row, on the keys that row sees
-      if (edge_tile) {
-        const SeqSpan& s = it.s;
-        const int n_edge = span_edges(s), n_low = s.lo - s.lo0;
-        if (tid < n_edge) {
-          const int j = tid < n_low ? s.lo0 + tid : s.hi + tid - n_low;
-          const int row = cache_row(p.pages, it.b, j);
-          if (row < 0 && p.status) atomicCAS(p.status, 0, IQ_ERR_ROUTE);
-          edge_rows[tid] = row;
-        }
-        __syncthreads();
-        constexpr int PER = G::DP / 32;
-        float* edge_o = join;                    // [RB][DP]
-        float* edge_ml = join + G::RB * G::DP;   // [RB][2]
-        for (int rr = warp; rr < G::RB; rr += G::W) {
-          const int r = r0 + rr;
-          if (r >= p.rows_all) break;
-          const int tok = r / p.group, head = h * p.group + r % p.group;
-          const int pos = s.n - p.q_len + tok;
-          const __nv_bfloat16* src = p.q + it.b * p.q_b + tok * p.q_r + head * p.q_h;
-          float qv[PER], ov[PER];
-#pragma unroll
-          for (int x = 0; x < PER; ++x) {
-            const int d = lane * PER + x;
-            qv[x] = d < p.dim ? __bfloat162float(src[d]) : 0.f;
-            ov[x] = 0.f;
-          }
-          float em = -INFINITY, el = 0.f;
-          for (int e = 0; e < n_edge; ++e) {
-            const int j = e < n_low ? s.lo0 + e : s.hi + e - n_low;
-            const bool visible = j <= pos && (p.window == 0 || j > pos - p.window);
-            float x = -INFINITY;
-            const int row = edge_rows[e];
-            if (visible) {
-              float dot = 0.f;
-              const uint8_t* kr = p.k + static_cast<long long>(max(row, 0)) * p.k_row + h * p.k_head;
-#pragma unroll
-              for (int y = 0; y < PER; ++y) {
-                const int d = lane * PER + y;
-                if (d < p.dim && row >= 0)
-                  dot += qv[y] * (G::KV == IQ_ACT_BF16
-                                      ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(kr)[d])
-                                      : e4m3_to_f32(kr[d]));
-              }
-              x = warp_sum(dot) * p.scale_log2;
-              const float top = fmaxf(em, x), u = top == -INFINITY ? 0.f : top;
-              const float f = ex2(em - u), w = ex2(x - u);
-              em = top;
-              el = el * f + w;
-              const uint8_t* vr = p.v + static_cast<long long>(max(row, 0)) * p.v_row + h * p.v_head;
-#pragma unroll
-              for (int y = 0; y < PER; ++y) {
-                const int d = lane * PER + y;
-                const float val = d < p.dim && row >= 0
-                                      ? (G::KV == IQ_ACT_BF16
-                                             ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(vr)[d])
-                                             : e4m3_to_f32(vr[d]))
-                                      : 0.f;
-                ov[y] = ov[y] * f + w * val;
+              for (int x = 0; x < MX; ++x) {
+                const float(&a)[4] = acc[nb][part * MX + x];
+                *reinterpret_cast<float4*>(mine + 128 * (x + 1)) = make_float4(a[0], a[1], a[2], a[3]);
               }
             }
-            if (p.scores && lane == 0)
-              p.scores[((static_cast<long long>(it.b) * p.kv_heads + h) * p.score_rows + j) *
-                           p.rows_pad + r] = x;
-          }
+            sync_all();
+            if (kg < half) {
+              if (part == 0) {
+                const float4 o4 = *reinterpret_cast<const float4*>(mine);
+                const float om[2] = {o4.x, o4.y}, ol[2] = {o4.z, o4.w};
 #pragma unroll
-          for (int x = 0; x < PER; ++x) edge_o[rr * G::DP + lane * PER + x] = ov[x];
-          if (lane == 0) {
-            edge_ml[2 * rr] = em;
-            edge_ml[2 * rr + 1] = el;
-          }
-        }
-        __syncthreads();
-        have_edges = true;
-      }
-      if (kg == 0) {
-        const bool whole = unit_end && seg_first_tile == 0;
-        const int slot_out = 2 * cta + (seg_first_tile == 0 ? 1 : 0);
-#pragma unroll
-        for (int nb = 0; nb < G::NBW; ++nb) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const int rr = (wr * G::NBW + nb) * 8 + 2 * t + c, r = r0 + rr;
-            if (r >= p.rows_all) continue;
-            float f = 1.f, e = 0.f;
-            if (have_edges) {
-              const float om = join[G::RB * G::DP + 2 * rr], ol = join[G::RB * G::DP + 2 * rr + 1];
-              const float top = fmaxf(m[nb][c], om), uu = top == -INFINITY ? 0.f : top;
-              f = ex2(m[nb][c] - uu);
-              e = ex2(om - uu);
-              m[nb][c] = top;
-              l[nb][c] = l[nb][c] * f + ol * e;
-            }
-            const float inv = l[nb][c] > 0.f ? 1.f / l[nb][c] : (l[nb][c] == 0.f ? 0.f : l[nb][c]);
-            const int tok = r / p.group, head = h * p.group + r % p.group;
-            __nv_bfloat16* o = p.out + it.b * p.o_b + tok * p.o_r + head * p.o_h;
-            float* po = p.part + (static_cast<size_t>(slot_out) * G::RB + rr) * G::DP;
-#pragma unroll
-            for (int x = 0; x < G::MT; ++x) {
-#pragma unroll
-              for (int y = 0; y < 2; ++y) {      // rows g and g + 8 of the m-tile
-                int d;
-                if (G::KV == IQ_ACT_BF16) d = 16 * x + 8 * y + g;
-                else d = G::DP >= 128 ? (x / 8) * 128 + g * 16 + 2 * (x % 8) + y : g * 8 + 2 * x + y;
-                float val = acc[nb][x][2 * y + c];
-                if (have_edges) val = val * f + e * join[rr * G::DP + d];
-                if (whole) {
-                  if (d < p.dim) o[d] = __float2bfloat16_rn(val * inv);
-                } else {
-                  po[d] = val;
+                for (int c = 0; c < 2; ++c) {
+                  const float top = fmaxf(m[nb][c], om[c]), u = top == -INFINITY ? 0.f : top;
+                  f[c] = ex2(m[nb][c] - u);
+                  e[c] = ex2(om[c] - u);
+                  m[nb][c] = top;
+                  l[nb][c] = l[nb][c] * f[c] + ol[c] * e[c];
                 }
               }
+#pragma unroll
+              for (int x = 0; x < MX; ++x) {
+                const float4 v = *reinterpret_cast<const float4*>(mine + 128 * (x + 1));
+                float(&a)[4] = acc[nb][part * MX + x];
+                a[0] = a[0] * f[0] + v.x * e[0];
+                a[1] = a[1] * f[1] + v.y * e[1];
+                a[2] = a[2] * f[0] + v.z * e[0];
+                a[3] = a[3] * f[1] + v.w * e[1];
+              }
             }
-            if (g == 0) {
-              if (whole) {
-                const float z = l[nb][c] > 0.f ? m[nb][c] + log2f(l[nb][c])
-                                               : (l[nb][c] == 0.f ? -INFINITY : l[nb][c]);
-                const long long at = (static_cast<long long>(it.b) * p.q_len + tok) * p.q_heads + head;
-                if (p.lse) p.lse[at] = z * kLn2;
-                if (p.lse2) p.lse2[at] = z;
-              } else {
-                p.part_ml[static_cast<size_t>(slot_out) * G::RB + rr] = make_float2(m[nb][c], l[nb][c]);
+            sync_all();
+          }
+        }
+      }
+      const bool whole = unit_end && from_start;
+      const int slot_out = 2 * cta + (from_start ? 1 : 0);
+      if (unit_end && tid == 0) p.units[it.b * per + it.hb].y = cta;
+      if (kg == 0) {
+#pragma unroll
+        for (int nb = 0; nb < G::NBW; ++nb) {
+          const int block = wr * G::NBW + nb;    // rows 8 block .. + 7 of the unit
+          float inv[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            inv[c] = l[nb][c] > 0.f ? 1.f / l[nb][c] : (l[nb][c] == 0.f ? 0.f : l[nb][c]);
+            const int r = r0 + block * 8 + 2 * t + c;
+            if (g != 0 || r >= p.rows_all) continue;
+            if (whole) {
+              const float z = l[nb][c] > 0.f ? m[nb][c] + log2f(l[nb][c])
+                                             : (l[nb][c] == 0.f ? -INFINITY : l[nb][c]);
+              const int tok = r / p.group, head = h * p.group + r - tok * p.group;
+              const long long at = (static_cast<long long>(it.b) * p.q_len + tok) * p.q_heads + head;
+              if (p.lse) p.lse[at] = z * kLn2;
+              if (p.lse2) p.lse2[at] = z;
+            } else {
+              p.part_ml[(static_cast<size_t>(slot_out) * G::HG + hg) * G::RB + block * 8 + 2 * t + c] =
+                  make_float2(m[nb][c], l[nb][c]);
+            }
+          }
+          if (!whole) {                          // fragments as they are
+            float4* dst = reinterpret_cast<float4*>(p.part) +
+                          ((static_cast<size_t>(slot_out) * G::HG + hg) * (G::RB / 8) + block) * G::MT * 32 + lane;
+#pragma unroll
+            for (int x = 0; x < G::MT; ++x)
+              dst[x * 32] = make_float4(acc[nb][x][0], acc[nb][x][1], acc[nb][x][2], acc[nb][x][3]);
+          } else if (G::KV == IQ_ACT_BF16) {
+            // transposed back: lane (g, t) writes channels 2t, 2t + 1 of row g of each 8 x 8
+            const int r = r0 + block * 8 + g, tok = r / p.group, head = h * p.group + r - tok * p.group;
+            __nv_bfloat16* o = p.out + it.b * p.o_b + tok * p.o_r + head * p.o_h + 2 * t;
+#pragma unroll
+            for (int x = 0; x < G::MT; ++x) {
+              const uint32_t lo = transpose8x8(pack_bf16(acc[nb][x][0] * inv[0], acc[nb][x][1] * inv[1]));
+              const uint32_t hi = transpose8x8(pack_bf16(acc[nb][x][2] * inv[0], acc[nb][x][3] * inv[1]));
+              if (r < p.rows_all && 16 * x < p.dim) {
+                *reinterpret_cast<uint32_t*>(o + 16 * x) = lo;
+                *reinterpret_cast<uint32_t*>(o + 16 * x + 8) = hi;
+              }
+            }
+          } else {
+            // lane (g, t) holds runs of 16 (D = 64: 8) channels of rows 2t and 2t + 1
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const int r = r0 + block * 8 + 2 * t + c;
+              if (r >= p.rows_all) continue;
+              const int tok = r / p.group, head = h * p.group + r - tok * p.group;
+              __nv_bfloat16* o = p.out + it.b * p.o_b + tok * p.o_r + head * p.o_h;
+#pragma unroll
+              for (int x = 0; x < G::MT; x += 4) {
+                const int d = channel_of<G>(x, 0, g);
+                uint4 w;
+                w.x = pack_bf16(acc[nb][x][c] * inv[c], acc[nb][x][2 + c] * inv[c]);
+                w.y = pack_bf16(acc[nb][x + 1][c] * inv[c], acc[nb][x + 1][2 + c] * inv[c]);
+                w.z = pack_bf16(acc[nb][x + 2][c] * inv[c], acc[nb][x + 2][2 + c] * inv[c]);
+                w.w = pack_bf16(acc[nb][x + 3][c] * inv[c], acc[nb][x + 3][2 + c] * inv[c]);
+                if (d < p.dim) *reinterpret_cast<uint4*>(o + d) = w;
               }
             }
           }
         }
       }
-      __syncthreads();                           // the join buffer is free again
+      if (p.q_len > 1) {
+        sync_all();
+        if (*not_finite) {
+          add_not_finite<G>(p, it.b, it.n, it.h0, r0, seg_key, it.j + G::TK, whole, slot_out);
+          sync_all();
+          if (tid == 0) *not_finite = 0;
+        }
+      }
+      if (G::KG > 1 || G::QS || p.q_len > 1) sync_all();   // the shared buffers are free again
       fresh = true;
+      from_start = true;
     }
-    iter_next<G>(it, p, prefix, lens);
+    it.next(p, prefix, lens, per);
   }
-  cp_async_wait<0>();
 }
 
 // ------------------------------------------------------------------------------------
 // Adds the partial results of the units that several CTAs shared: slot 2c + 1 of the first
-// CTA, slot 2c of the others, in that order.  `wide`: a block of eight warps a query row
-// (many partials a unit); else a warp a row.
+// CTA, slot 2c of the others, in that order.  A block joins eight query rows of a head, a
+// thread the four values of one lane of an m-tile; WIDE (many partial results a unit): a
+// block joins one m-tile, its eight warps every eighth partial result.  It is all latency
+// (the unit's place, then its partial results), so a thread has all its loads in flight at
+// once, those of the maxima and sums among them.
 constexpr int kJoinThreads = 256;
+constexpr int kJoinParts = 160;                  // partial results of a unit, at most (one a CTA)
 
-template <int DP, int RB>
-__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_constant__ AttnParams p,
-                                                                int wide) {
-  __shared__ float red_ml[8][2];
-  __shared__ float red_o[8][DP];
-  constexpr int PER = DP / 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int per = p.kv_heads * p.n_rb;
-  const int u = blockIdx.x;
-  const int b = u / per, hb = u - b * per, h = hb / p.n_rb, r0 = (hb - h * p.n_rb) * RB;
-  const int rr = wide ? blockIdx.y : blockIdx.y * 8 + warp;
-  const int r = r0 + rr;
+template <class G, bool WIDE>
+__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_constant__ AttnParams p) {
+  __shared__ float fac[8][kJoinParts];
+  __shared__ float stat[8];
+  __shared__ float4 red[8][32];
+  constexpr int BATCH = WIDE ? kJoinParts / 8 : 8;   // loads of a thread in flight
+  constexpr int EACH = kJoinParts / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int per = p.kv_heads / G::HG * p.n_rb;
+  const int u = blockIdx.x / G::HG, hg = blockIdx.x % G::HG;
+  const int b = u / per, hb = u - b * per, h = hb / p.n_rb * G::HG + hg;
+  const int block = blockIdx.y, r0 = hb % p.n_rb * G::RB + block * 8;
   pdl_wait();
   pdl_launch_dependents();
-  const int2 c = p.units[u];
-  if (c.y <= c.x || (wide && r >= p.rows_all)) return;
-  const bool live = rr < RB && r < p.rows_all;
-  float M = -INFINITY, L = 0.f, o[PER];
+  const int2 c = __ldcg(p.units + u);
+  const int n = c.y - c.x + 1;
+  if (n <= 1 || r0 >= p.rows_all) return;
+  auto slot_of = [&](int k) { return (2 * (c.x + k) + (k == 0 ? 1 : 0)) * G::HG + hg; };
+  const float4* part = reinterpret_cast<const float4*>(p.part) + block * G::MT * 32 + lane;
+  auto load = [&](int x, int k) {
+    return __ldcg(part + static_cast<size_t>(slot_of(k)) * (G::RB / 8) * G::MT * 32 + x * 32);
+  };
+  const int step = WIDE ? 8 : 1, first = WIDE ? warp : 0;
+  float4 v[BATCH];
+  const int x0 = WIDE ? blockIdx.z : warp;
 #pragma unroll
-  for (int x = 0; x < PER; ++x) o[x] = 0.f;
-  if (live) {
-    const int step = wide ? 8 : 1, n = c.y - c.x + 1;
-    for (int base = wide ? warp : 0; base < n; base += 32 * step) {
-      const int mine = base + lane * step;
-      auto slot_of = [&](int k) { return static_cast<size_t>(2 * (c.x + k) + (k == 0 ? 1 : 0)) * RB + rr; };
-      float2 ml = make_float2(-INFINITY, 0.f);
-      if (mine < n) ml = __ldcg(p.part_ml + slot_of(mine));
-      const float top = fmaxf(M, warp_max(ml.x)), uu = top == -INFINITY ? 0.f : top;
-      const float old = ex2(M - uu), f = ex2(ml.x - uu);
-      M = top;
-      L = L * old + warp_sum(ml.y * f);
+  for (int i = 0; i < BATCH; ++i)
+    if (x0 < G::MT && first + i * step < n) v[i] = load(x0, first + i * step);
+  // ---- warp w: row w's maximum, sum and each partial result's factor
+  {
+    const bool live = r0 + warp < p.rows_all;
+    const float2* ml = p.part_ml + block * 8 + warp;
+    float2 z[EACH];
+    float top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int x = 0; x < PER; ++x) o[x] *= old;
-      const int cnt = min(32, (n - base + step - 1) / step);
-#pragma unroll 8
-      for (int k = 0; k < cnt; ++k) {
-        const float fk = __shfl_sync(0xffffffffu, f, k);
-        const float* src = p.part + slot_of(base + k * step) * DP + lane * PER;
-        float v[PER];
-        if constexpr (PER >= 4) {
+    for (int i = 0; i < EACH; ++i) {
+      z[i] = make_float2(-INFINITY, 0.f);
+      if (live && lane + 32 * i < n) z[i] = __ldcg(&ml[static_cast<size_t>(slot_of(lane + 32 * i)) * G::RB]);
+    }
 #pragma unroll
-          for (int x = 0; x < PER; x += 4) {
-            const float4 w = __ldcg(reinterpret_cast<const float4*>(src + x));
-            v[x] = w.x; v[x + 1] = w.y; v[x + 2] = w.z; v[x + 3] = w.w;
-          }
-        } else {
-          const float2 w = __ldcg(reinterpret_cast<const float2*>(src));
-          v[0] = w.x; v[1] = w.y;
-        }
+    for (int i = 0; i < EACH; ++i) top = fmaxf(top, z[i].x);
+    top = warp_max(top);
+    const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int x = 0; x < PER; ++x) o[x] += fk * v[x];
+    for (int i = 0; i < EACH; ++i) {
+      const float f = ex2(z[i].x - base);
+      fac[warp][lane + 32 * i] = f;
+      sum += f * z[i].y;
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) {
+      stat[warp] = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);
+      if (live && (!WIDE || blockIdx.z == 0)) {
+        const float y = sum > 0.f ? top + log2f(sum) : (sum == 0.f ? -INFINITY : sum);
+        const int r = r0 + warp, tok = r / p.group, head = h * p.group + r - tok * p.group;
+        const long long at = (static_cast<long long>(b) * p.q_len + tok) * p.q_heads + head;
+        if (p.lse) p.lse[at] = y * kLn2;
+        if (p.lse2) p.lse2[at] = y;
       }
     }
   }
-  if (wide) {
-    if (lane == 0) { red_ml[warp][0] = M; red_ml[warp][1] = L; }
+  __syncthreads();
+  auto put = [&](int x, float4 o) {
+    const float val[2][2] = {{o.x, o.z}, {o.y, o.w}};
 #pragma unroll
-    for (int x = 0; x < PER; ++x) red_o[warp][lane * PER + x] = o[x];
-    __syncthreads();
-    if (warp) return;
-    float top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, red_ml[w][0]);
-    const float uu = top == -INFINITY ? 0.f : top;
-    L = 0.f;
-#pragma unroll
-    for (int x = 0; x < PER; ++x) o[x] = 0.f;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      const float f = ex2(red_ml[w][0] - uu);
-      L += f * red_ml[w][1];
-#pragma unroll
-      for (int x = 0; x < PER; ++x) o[x] += f * red_o[w][lane * PER + x];
+    for (int y = 0; y < 2; ++y) {
+      const int r = r0 + 2 * t + y;
+      if (r >= p.rows_all) continue;
+      const int tok = r / p.group, head = h * p.group + r - tok * p.group;
+      __nv_bfloat16* dst = p.out + b * p.o_b + tok * p.o_r + head * p.o_h;
+      const float inv = stat[2 * t + y];
+      const int d0 = channel_of<G>(x, 0, g), d1 = channel_of<G>(x, 1, g);
+      if (d0 < p.dim) dst[d0] = __float2bfloat16_rn(val[y][0] * inv);
+      if (d1 < p.dim) dst[d1] = __float2bfloat16_rn(val[y][1] * inv);
     }
-    M = top;
-  }
-  if (!live) return;
-  const int tok = r / p.group, head = h * p.group + r % p.group;
-  __nv_bfloat16* dst = p.out + b * p.o_b + tok * p.o_r + head * p.o_h;
-  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+  };
+#pragma unroll 1
+  for (int x = x0; x < G::MT; x += WIDE ? G::MT : 8) {
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int k0 = first; k0 < n; k0 += BATCH * step) {
+      if (x != x0 || k0 != first)
 #pragma unroll
-  for (int x = 0; x < PER; ++x)
-    if (lane * PER + x < p.dim) dst[lane * PER + x] = __float2bfloat16_rn(o[x] * inv);
-  if (lane == 0) {
-    const float z = L > 0.f ? M + log2f(L) : (L == 0.f ? -INFINITY : L);
-    const long long at = (static_cast<long long>(b) * p.q_len + tok) * p.q_heads + head;
-    if (p.lse) p.lse[at] = z * kLn2;
-    if (p.lse2) p.lse2[at] = z;
+        for (int i = 0; i < BATCH; ++i)
+          if (k0 + i * step < n) v[i] = load(x, k0 + i * step);
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int k = k0 + i * step;
+        if (k < n) {
+          const float f0 = fac[2 * t][k], f1 = fac[2 * t + 1][k];
+          o.x += f0 * v[i].x;
+          o.y += f1 * v[i].y;
+          o.z += f0 * v[i].z;
+          o.w += f1 * v[i].w;
+        }
+      }
+    }
+    if (!WIDE) put(x, o);
+    else red[warp][lane] = o;
   }
+  if (!WIDE) return;
+  __syncthreads();
+  if (warp) return;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const float4 a = red[w][lane];
+    o.x += a.x; o.y += a.y; o.z += a.z; o.w += a.w;
+  }
+  put(x0, o);
 }
 
 // ------------------------------------------------------------------------------------
@@ -876,7 +1210,7 @@ __global__ void __launch_bounds__(256) attn_weights_kernel(const __grid_constant
     z[r] = v;
   }
   __syncthreads();
-  for (int j = s.lo0 + blockIdx.x * blockDim.x + threadIdx.x; j < s.n; j += gridDim.x * blockDim.x) {
+  for (int j = s.lo + blockIdx.x * blockDim.x + threadIdx.x; j < s.n; j += gridDim.x * blockDim.x) {
     const float* src = p.scores +
                        ((static_cast<long long>(b) * p.kv_heads + h) * p.score_rows + j) * p.rows_pad;
     float w = 0.f;
@@ -953,22 +1287,35 @@ static int attn_launch(K kernel, dim3 grid, int threads, int smem, void* stream,
 struct AttnWork {
   size_t part, part_ml, units, lse2, scores, total;
 };
-constexpr int kAttnMaxCtas = 2 * 160;            // CTAs of the split kernel, at most
+constexpr int kAttnMaxCtas = 160;                // CTAs of the split kernel, at most
 
-static int pad_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
+// (64-byte rows are copied in boxes of two rows at least: a box starts on 128 bytes)
+static int pad_dim(int d, int elt, int page) {
+  return d <= 64 && (elt == 2 || page % 2 == 0) ? 64 : d <= 128 ? 128 : 256;
+}
 static int block_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+// Heads a unit.  Neighbouring heads' rows are one piece of DRAM: against one head a unit, four
+// took a ragged bf16 batch (32 / 8 heads) from 205 to 150 us and 32 x 8192 rows of e4m3 from
+// 135 to 91; eight leave as many more partial results to join (128k rows of e4m3: 54 us, four
+// 51).  No more than the rings of the geometry that the rows take.
+static int head_group(int kv_heads, int rb, int dim) {
+  int g = dim > 128 ? (rb <= 16 ? 4 : rb <= 32 ? 2 : 1) : (rb <= 32 ? 4 : 2);
+  while (kv_heads % g) g /= 2;
+  return g;
+}
 
 static AttnWork attn_work(int batch, int q_len, int q_heads, int kv_heads, int dim, int rows,
                           bool weights) {
   const int all = q_heads / kv_heads * q_len;
-  const int rb = block_rows(all), n_rb = (all + rb - 1) / rb;
+  const int rb = block_rows(all), n_rb = (all + rb - 1) / rb, rows_cta = rb * head_group(kv_heads, rb, dim);
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   AttnWork w{};
   size_t at = 0;
   w.part = at;
-  at += up(static_cast<size_t>(2 * kAttnMaxCtas) * rb * pad_dim(dim) * 4);
+  at += up(static_cast<size_t>(2 * kAttnMaxCtas) * rows_cta * (dim <= 128 ? 128 : 256) * 4);
   w.part_ml = at;
-  at += up(static_cast<size_t>(2 * kAttnMaxCtas) * rb * 8);
+  at += up(static_cast<size_t>(2 * kAttnMaxCtas) * rows_cta * 8);
   w.units = at;
   at += up(static_cast<size_t>(batch) * kv_heads * n_rb * 8);
   if (weights) {
@@ -987,35 +1334,110 @@ static bool attn_shape_ok(int batch, int q_len, int q_heads, int kv_heads, int d
          dim >= 16 && dim <= 256 && dim % 16 == 0 && rows >= 1 && kv_heads <= 65535;
 }
 
+// The cache as (bytes of a head's row, rows, heads), in boxes of `pitch` bytes x box_rows x
+// box_heads with the swizzle whose width the box has.  Encoded anew for every call (a few hundred
+// nanoseconds on the host): nothing is kept by address.
+static int attn_map(CUtensorMap* out, const void* base, const AttnParams& p, long long row,
+                    long long head, int elt, int pitch) {
+  typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                    const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                    const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                    CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<EncodeTiledFn> known{nullptr};
+  EncodeTiledFn encode = known.load();
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) !=
+            cudaSuccess || q != cudaDriverEntryPointSuccess || !fn)
+      return IQ_ERR_CUDA;
+    encode = reinterpret_cast<EncodeTiledFn>(fn);
+    known.store(encode);
+  }
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(p.dim * elt),
+                              static_cast<cuuint64_t>(p.pages.capacity),
+                              static_cast<cuuint64_t>(p.kv_heads)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.pages.capacity > 1 ? row : p.dim * elt),
+                                 static_cast<cuuint64_t>(p.kv_heads > 1 ? head : p.dim * elt)};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(pitch), static_cast<cuuint32_t>(p.box_rows),
+                             static_cast<cuuint32_t>(p.box_heads)};
+  const cuuint32_t ones[3] = {1, 1, 1};
+  const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims,
+                            strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            pitch == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    fprintf(stderr, "iqb200: cuTensorMapEncodeTiled failed (%d)\n", static_cast<int>(r));
+    return IQ_ERR_CUDA;
+  }
+  return IQ_OK;
+}
+
 template <class G>
 static int attn_run(AttnParams& p, int n_sm, bool pdl, void* stream) {
-  const long long tiles = static_cast<long long>(p.batch) * p.kv_heads * p.n_rb *
-                          ((p.max_rows + G::TK - 1) / G::TK + 1);
+  const long long tiles = static_cast<long long>(p.batch) * (p.kv_heads / G::HG) * p.n_rb *
+                          ((p.max_rows + G::TK - 1) / G::TK + 2);
   if (tiles > 0x7fffffffLL) return IQ_ERR_UNSUPPORTED;
-  const int grid = static_cast<int>(tiles < n_sm * G::CTAS ? tiles : n_sm * G::CTAS);
-  int rc = attn_launch(attn_kernel<G>, dim3(grid), G::THREADS, G::SMEM, stream, pdl, p);
+  int box = G::KPW;
+  while (p.pages.page % box) box /= 2;
+  p.box_rows = box;
+  p.box_heads = box == G::KPW ? G::HG : 1;       // (a stage's heads lie KPW rows apart)
+  // One warp issues the boxes, at some 60 ns each: past sixteen a tile the threads are faster
+  // (pages of 16 rows, 128k rows of e4m3: 54 us against 58; pages of one row need 64 a head).
+  // Boxes leave less to do per tile where there are few (4096 rows: 8.9 us against 11.4).
+  p.gather = 2 * G::BOXES * (G::KPW / box) * (G::HG / p.box_heads) * G::KG > 16;
+  if (G::MOVE_REGS) {                            // (a launch with fewer registers would wait for good)
+    static std::atomic<int> regs{0};
+    if (regs.load() == 0) {
+      cudaFuncAttributes at{};
+      if (cudaFuncGetAttributes(&at, attn_kernel<G>) != cudaSuccess) return IQ_ERR_CUDA;
+      regs.store(at.numRegs);
+    }
+    if (regs.load() < G::REGS) return IQ_ERR_CUDA;
+  }
+  int rc = attn_map(&p.k_map, p.k, p, p.k_row, p.k_head, G::ELT, G::PITCH);
+  if (rc == IQ_OK) rc = attn_map(&p.v_map, p.v, p, p.v_row, p.v_head, G::ELT, G::PITCH);
   if (rc != IQ_OK) return rc;
-  const int units = p.batch * p.kv_heads * p.n_rb;
-  // a unit's share of the CTAs: above eight, its partial results are worth a block a row
-  const int wide = grid > 8 * units;
-  const int y = wide ? (p.rows_all < G::RB ? p.rows_all : G::RB)
-                     : ((p.rows_all < G::RB ? p.rows_all : G::RB) + 7) / 8;
-  return attn_launch(attn_join_kernel<G::DP, G::RB>, dim3(units, y), kJoinThreads, 0, stream, true,
-                     p, wide);
+  const int grid = static_cast<int>(tiles < n_sm ? tiles : n_sm);
+  rc = attn_launch(attn_kernel<G>, dim3(grid), G::THREADS, G::SMEM, stream, pdl, p);
+  if (rc != IQ_OK) return rc;
+  const int heads = p.batch * p.kv_heads * p.n_rb;   // units x heads of a unit
+  const int blocks = ((p.rows_all < G::RB ? p.rows_all : G::RB) + 7) / 8;
+  // the CTAs that share a unit: from nine on its partial results are worth a block an m-tile
+  const int wide = static_cast<long long>(grid) * G::HG > 8LL * heads;
+  return wide ? attn_launch(attn_join_kernel<G, true>, dim3(heads, blocks, G::MT), kJoinThreads, 0, stream,
+                            true, p)
+              : attn_launch(attn_join_kernel<G, false>, dim3(heads, blocks), kJoinThreads, 0, stream, true, p);
+}
+
+// Sixteen rows a warp: their fragments of K and V are read and widened once.  Thirty-two (with
+// q in shared memory) left too few registers: 67 us against 37 for 32 rows over 32k keys of
+// e4m3, sixteen warps of eight rows 42.
+template <int KV, int DP, int HG>
+static int attn_pick_rows(AttnParams& p, int n_sm, bool pdl, void* stream) {
+  if constexpr (DP <= 128) {
+    if (p.rows_all <= 8) return attn_run<AttnGeo<KV, DP, 1, 1, HG, 8>>(p, n_sm, pdl, stream);
+    if (p.rows_all <= 16) return attn_run<AttnGeo<KV, DP, 2, 1, HG, 8>>(p, n_sm, pdl, stream);
+    if (p.rows_all <= 32) return attn_run<AttnGeo<KV, DP, 2, 2, HG, 8>>(p, n_sm, pdl, stream);
+    if constexpr (HG <= 2) return attn_run<AttnGeo<KV, DP, 2, 4, HG, 8>>(p, n_sm, pdl, stream);
+  } else {
+    constexpr int W = KV == IQ_ACT_BF16 ? 4 : 8;     // (two stages of eight rings do not fit)
+    if (p.rows_all <= 8) return attn_run<AttnGeo<KV, DP, 1, 1, HG, W>>(p, n_sm, pdl, stream);
+    if (p.rows_all <= 16) return attn_run<AttnGeo<KV, DP, 2, 1, HG, W>>(p, n_sm, pdl, stream);
+    if constexpr (HG <= 2) {
+      if (p.rows_all <= 32) return attn_run<AttnGeo<KV, DP, 2, 2, HG, 8>>(p, n_sm, pdl, stream);
+    }
+    if constexpr (HG == 1) return attn_run<AttnGeo<KV, DP, 2, 4, 1, 8>>(p, n_sm, pdl, stream);
+  }
+  return IQ_ERR_UNSUPPORTED;
 }
 
 template <int KV, int DP>
 static int attn_pick(AttnParams& p, int n_sm, bool pdl, void* stream) {
-  constexpr int W = KV == IQ_ACT_BF16 && DP == 256 ? 4 : 8;
-  if (p.rows_all <= 8) return attn_run<AttnGeo<KV, DP, 1, 1, W, 1>>(p, n_sm, pdl, stream);
-  if constexpr (DP <= 128) {
-    if (p.rows_all <= 16) return attn_run<AttnGeo<KV, DP, 2, 1, 8, 1>>(p, n_sm, pdl, stream);
-    if (p.rows_all <= 32) return attn_run<AttnGeo<KV, DP, 2, 2, 8, 1>>(p, n_sm, pdl, stream);
-    return attn_run<AttnGeo<KV, DP, 2, 4, 8, 1>>(p, n_sm, pdl, stream);
-  } else {
-    if (p.rows_all <= 16) return attn_run<AttnGeo<KV, DP, 1, 2, W, 1>>(p, n_sm, pdl, stream);
-    if (p.rows_all <= 32) return attn_run<AttnGeo<KV, DP, 1, 4, 8, 1>>(p, n_sm, pdl, stream);
-    return attn_run<AttnGeo<KV, DP, 1, 8, 8, 1>>(p, n_sm, pdl, stream);
+  switch (head_group(p.kv_heads, block_rows(p.rows_all), p.dim)) {
+    case 4: return attn_pick_rows<KV, DP, 4>(p, n_sm, pdl, stream);
+    case 2: return attn_pick_rows<KV, DP, 2>(p, n_sm, pdl, stream);
+    default: return attn_pick_rows<KV, DP, 1>(p, n_sm, pdl, stream);
   }
 }
 
@@ -1047,16 +1469,21 @@ extern "C" int iq_attn_decode(const iq_attn_args* a, void* stream) {
   const AttnWork w = attn_work(a->batch, a->q_len, a->q_heads, a->kv_heads, a->head_dim,
                                static_cast<int>(rows), weights);
   if (a->work_bytes < w.total) return IQ_ERR_ARG;
-  // 16-byte copies of cache rows, 4-byte loads of q
+  // 16-byte loads and stores
   const int64_t elt = a->kv_kind == IQ_ACT_BF16 ? 2 : 1;
   const uint64_t al = reinterpret_cast<uint64_t>(a->k_cache) | reinterpret_cast<uint64_t>(a->v_cache) |
                       static_cast<uint64_t>(a->k_row * elt) | static_cast<uint64_t>(a->k_head * elt) |
                       static_cast<uint64_t>(a->v_row * elt) | static_cast<uint64_t>(a->v_head * elt) |
                       reinterpret_cast<uint64_t>(a->work);
   if (al & 15) return IQ_ERR_ARG;
-  if ((reinterpret_cast<uint64_t>(a->q) & 3) || ((a->q_b | a->q_r | a->q_h) & 1)) return IQ_ERR_ARG;
+  const int64_t far = int64_t{1} << 40;          // a tensor map's strides, bytes
+  for (const int64_t st : {a->k_row, a->k_head, a->v_row, a->v_head})
+    if (st < 0 || st * elt >= far) return IQ_ERR_ARG;
+  if (((reinterpret_cast<uint64_t>(a->q) | reinterpret_cast<uint64_t>(a->out)) & 15) ||
+      ((a->q_b | a->q_r | a->q_h | a->o_b | a->o_r | a->o_h) & 7))
+    return IQ_ERR_ARG;
   const int n_sm = attn_sms();
-  if (n_sm == 0 || n_sm * 2 > kAttnMaxCtas) return IQ_ERR_CUDA;
+  if (n_sm == 0 || n_sm > kAttnMaxCtas) return IQ_ERR_CUDA;
 
   AttnParams p{};
   p.q = static_cast<const __nv_bfloat16*>(a->q);
@@ -1104,7 +1531,7 @@ extern "C" int iq_attn_decode(const iq_attn_args* a, void* stream) {
   }
   const bool bf16 = a->kv_kind == IQ_ACT_BF16, pdl = a->pdl != 0;
   int rc;
-  switch (pad_dim(a->head_dim)) {
+  switch (pad_dim(a->head_dim, static_cast<int>(elt), a->page_size)) {
     case 64:
       rc = bf16 ? attn_pick<IQ_ACT_BF16, 64>(p, n_sm, pdl, stream)
                 : attn_pick<IQ_ACT_E4M3, 64>(p, n_sm, pdl, stream);

@@ -1,5 +1,4 @@
-// What the kernels over the paged key/value cache share: the cache's geometry and copies
-// that fill with zeros.
+// What the kernels over the paged key/value cache share: the cache's geometry.
 #pragma once
 
 #include "common.cuh"
@@ -16,12 +15,17 @@ struct PageTable {
   int capacity;            // rows of the cache
 };
 
-__device__ __forceinline__ int cache_row(const PageTable& t, int b, int j) {
-  const int pg = t.shift >= 0 ? j >> t.shift : j / t.page;
-  const int off = j - pg * t.page;
-  const int id = __ldg(t.table + b * t.stride + pg);
+// The page that holds row j of sequence b, and the cache row of row j given its page.
+__device__ __forceinline__ int page_id(const PageTable& t, int b, int j) {
+  return __ldg(t.table + b * t.stride + (t.shift >= 0 ? j >> t.shift : j / t.page));
+}
+__device__ __forceinline__ int page_row(const PageTable& t, int id, int j) {
+  const int off = t.shift >= 0 ? j & (t.page - 1) : j % t.page;
   const long long row = static_cast<long long>(id) * t.page + off;
   return id >= 0 && row < t.capacity ? static_cast<int>(row) : -1;
+}
+__device__ __forceinline__ int cache_row(const PageTable& t, int b, int j) {
+  return page_row(t, page_id(t, b, j), j);
 }
 
 // 16 bytes global -> shared; `ok` false fills with zeros and reads nothing.
@@ -29,13 +33,6 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool o
   const int n = ok ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
                : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 // 2^x, flushing results below the smallest normal number (relative error <= 2^-22).

@@ -430,13 +430,13 @@ def _strided(name, t, dtype, shape, dev, written=False):
     return st
 
 
-def _cache_pair(k_cache, v_cache, dev, written=False):
+def _cache_pair(k_cache, v_cache, dev):
     if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 3:
         raise ValueError("the KV caches must be [capacity, kv_heads, head_dim] tensors")
     if k_cache.dtype != torch.bfloat16 and k_cache.dtype != E4M3:
         raise ValueError("the KV caches must both be bf16 or both e4m3")
-    ks = _strided("k_cache", k_cache, k_cache.dtype, k_cache.shape, dev, written)
-    vs = _strided("v_cache", v_cache, k_cache.dtype, k_cache.shape, dev, written)
+    ks = _strided("k_cache", k_cache, k_cache.dtype, k_cache.shape, dev, True)
+    vs = _strided("v_cache", v_cache, k_cache.dtype, k_cache.shape, dev, True)
     return ks, vs
 
 
@@ -578,7 +578,7 @@ def kv_evict(k_cache, v_cache, page_table, lengths, weights, positions, seen, *,
     dev = weights.device
     batch, kv_heads, n = weights.shape
     a = _lib.EvictArgs()
-    ks, vs = _cache_pair(k_cache, v_cache, dev, True)
+    ks, vs = _cache_pair(k_cache, v_cache, dev)
     capacity, kh, d = k_cache.shape
     rows = _paging(a, page_table, page_size, batch, dev)
     if kh != kv_heads or n < rows:

@@ -2,13 +2,13 @@
 // (iq_kv_evict) and the next tokens' rows (iq_kv_advance).
 //
 // Eviction is a selection and a movement.  The selection finds the budget-th largest of a
-// (sequence, head)'s weights exactly: order-preserving integers of the weights, four
-// histogram passes of eight bits each.  One cluster holds all of a head's weights in the
-// shared memory of its CTAs, so global memory is read once; a pass costs a histogram of
-// local words, one cluster barrier and the sum of the CTAs' 256 bins through distributed
-// shared memory.  The movement fills the freed places below the budget with the kept rows
-// above it: sources and destinations are disjoint, so it runs in place, in any order and on
-// all SMs, and moves the fewest rows there are to move.
+// (sequence, head)'s weights exactly: order-preserving integers of the weights, histogram
+// passes of 11, 11 and 10 bits (it stops at the pass whose bin is kept whole).  One cluster
+// holds all of a head's weights in the shared memory of its CTAs, so global memory is read
+// once; a pass costs a histogram of local words, one barrier and the sum of the CTAs' bins
+// through distributed shared memory.  The movement fills the freed places below the budget
+// with the kept rows above it: sources and destinations are disjoint, so it runs in place, in
+// any order and on all SMs, and moves the fewest rows there are to move.
 // What bounds it: latency (barriers, passes) for a step's few rows, HBM for a long prompt's.
 #include <math.h>
 #include <stdio.h>
@@ -24,7 +24,7 @@ namespace iqb {
 
 namespace cg = cooperative_groups;
 
-constexpr int kEvictThreads = 512;
+constexpr int kEvictThreads = 1024;
 constexpr int kEvictChunk = 32768;               // weights a CTA of a cluster holds at most
 constexpr int kEvictCluster = 8;
 constexpr int kEvictRows = kEvictChunk * kEvictCluster;
@@ -73,201 +73,248 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 // Exclusive sum of `x` over the block's threads in thread order; *all gets the total.
-__device__ __forceinline__ int block_scan(int x, int* sums /* [33] */, int* all) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  int incl = x;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
-  }
-  __syncthreads();                               // `sums` may still be read by an earlier scan
-  if (lane == 31) sums[warp] = incl;
-  __syncthreads();
-  if (warp == 0) {
-    const int v = lane < warps ? sums[lane] : 0;
-    int s = v;
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* sums /* [32] */, uint32_t* all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto inclusive = [&](uint32_t v) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += y;
+      const uint32_t y = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += y;
     }
-    if (lane < warps) sums[lane] = s - v;
-    if (lane == 31) sums[32] = s;
-  }
+    return v;
+  };
+  const uint32_t incl = inclusive(x);
+  if (lane == 31) sums[warp] = incl;
   __syncthreads();
-  *all = sums[32];
-  return incl - x + sums[warp];
+  const uint32_t warps = inclusive(sums[lane]);  // (every warp for itself)
+  const uint32_t before = __shfl_sync(0xffffffffu, warps, warp ? warp - 1 : 0);
+  *all = __shfl_sync(0xffffffffu, warps, 31);
+  __syncthreads();                               // `sums` is free again
+  return incl - x + (warp ? before : 0u);
 }
 
-// One cache row of K and of V, 16 bytes a thread of `width` threads.
-__device__ __forceinline__ void move_row(const EvictParams& p, int b, int h, int2 mv, int at, int width) {
-  const int to = cache_row(p.pages, b, mv.x), from = cache_row(p.pages, b, mv.y);
-  if (to < 0 || from < 0) {
-    if (p.status) atomicCAS(p.status, 0, IQ_ERR_ROUTE);
-    return;
-  }
-  for (int c = at * 16; c < p.row_bytes; c += width * 16) {
-    const uint4 k = *reinterpret_cast<const uint4*>(p.k + from * p.k_row + h * p.k_head + c);
-    const uint4 v = *reinterpret_cast<const uint4*>(p.v + from * p.v_row + h * p.v_head + c);
-    *reinterpret_cast<uint4*>(p.k + to * p.k_row + h * p.k_head + c) = k;
-    *reinterpret_cast<uint4*>(p.v + to * p.v_row + h * p.v_head + c) = v;
+// Moves [i0, i0 + step, ..) of `total`, a cache row of K and of V each, by groups of `width`
+// threads (16 bytes a thread), four moves in flight a group: a move is a chain of its list
+// entry, two page lookups and the row itself.
+__device__ __forceinline__ void move_rows(const EvictParams& p, int b, int h, const int2* moves, int i0,
+                                          int step, int total, int at, int width) {
+  constexpr int U = 4;
+#pragma unroll 1
+  for (int i = i0; i < total; i += U * step) {
+    int to[U], from[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      to[u] = from[u] = -1;
+      if (i + u * step < total) {
+        const int2 mv = __ldcg(moves + i + u * step);
+        to[u] = cache_row(p.pages, b, mv.x);
+        from[u] = cache_row(p.pages, b, mv.y);
+        if ((to[u] < 0 || from[u] < 0) && p.status) atomicCAS(p.status, 0, IQ_ERR_ROUTE);
+      }
+    }
+#pragma unroll 1
+    for (int c = at * 16; c < p.row_bytes; c += width * 16) {
+      uint4 k[U], v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (to[u] < 0 || from[u] < 0) continue;
+        k[u] = *reinterpret_cast<const uint4*>(p.k + from[u] * p.k_row + h * p.k_head + c);
+        v[u] = *reinterpret_cast<const uint4*>(p.v + from[u] * p.v_row + h * p.v_head + c);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (to[u] < 0 || from[u] < 0) continue;
+        *reinterpret_cast<uint4*>(p.k + to[u] * p.k_row + h * p.k_head + c) = k[u];
+        *reinterpret_cast<uint4*>(p.v + to[u] * p.v_row + h * p.v_head + c) = v[u];
+      }
+    }
   }
 }
 
 __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const __grid_constant__ EvictParams p) {
   extern __shared__ uint32_t keys[];             // [chunk]
-  __shared__ uint32_t hist[4][256];
-  __shared__ uint32_t bins[2][256];
-  __shared__ int sums[33];
-  __shared__ int found[2];                       // the digit, and what is still needed inside it
-  __shared__ int counts[3];                      // this CTA's equal keys, free places, moved rows
+  __shared__ uint32_t hist[3][2048];
+  __shared__ uint32_t sums[32];
+  __shared__ uint32_t places[kEvictThreads];     // a warp's flags in a round of keys; then what lies before
+  __shared__ uint32_t equals[kEvictThreads];
+  __shared__ uint32_t found[3];                  // the digit, what is needed inside it, and all it has
+  __shared__ uint32_t counts[2];                 // this CTA's keys at the edge; free places | moved rows << 16
   cg::cluster_group cluster = cg::this_cluster();
   const int cs = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int unit = blockIdx.x / cs, b = unit / p.kv_heads, h = unit - b * p.kv_heads;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto sync = [&]() {
+    if (cs == 1) __syncthreads();
+    else cluster.sync();
+  };
 
+#pragma unroll
+  for (int i = tid; i < 3 * 2048; i += kEvictThreads) hist[0][i] = 0;
   pdl_wait();
   pdl_launch_dependents();
-  const int n = evict_length(p, b, h == 0 && rank == 0 && tid == 0);
-  const int keep = min(n, p.budget);
-  if (h == 0 && rank == 0 && tid == 0) p.lengths_out[b] = keep;
+  // This CTA's rows; their weights and positions are on their way before the length is known
+  // (rows past it are inside the arrays).
+  const int i0 = rank * p.chunk, end = min(p.max_rows, i0 + p.chunk) - i0;
   const float* w = p.w + b * p.w_b + h * p.w_h;
   const int* pos = p.pos + b * p.p_b + h * p.p_h;
   float* w_out = p.w_out + b * p.wo_b + h * p.wo_h;
   int* pos_out = p.pos_out + b * p.po_b + h * p.po_h;
+  constexpr int AHEAD = 8;
+  float wv[AHEAD];
+  int pv[AHEAD];
+#pragma unroll
+  for (int x = 0; x < AHEAD; ++x) {
+    const int i = tid + x * kEvictThreads;
+    if (i < end) {
+      wv[x] = w[i0 + i];
+      pv[x] = pos[i0 + i];
+    }
+  }
+  const int n = evict_length(p, b, h == 0 && rank == 0 && tid == 0);
+  const int last = __ldg(p.seen + b) - p.keep_last;
+  const int keep = min(n, p.budget), mine = max(0, min(n - i0, end));
+  if (h == 0 && rank == 0 && tid == 0) p.lengths_out[b] = keep;
+  // The keys, and (out of place) the copies of what may stay below the budget; the places
+  // about to be filled get their old values too, before the moves below
+  auto take = [&](int i, float x, int at) {
+    keys[i] = at < p.keep_first || at >= last ? 0xffffffffu : weight_key(x);
+    if (i0 + i < keep) {
+      if (w_out != w) w_out[i0 + i] = x;
+      if (pos_out != pos) pos_out[i0 + i] = at;
+    }
+  };
+#pragma unroll
+  for (int x = 0; x < AHEAD; ++x)
+    if (tid + x * kEvictThreads < mine) take(tid + x * kEvictThreads, wv[x], pv[x]);
+#pragma unroll 4
+  for (int i = tid + AHEAD * kEvictThreads; i < mine; i += kEvictThreads) take(i, w[i0 + i], pos[i0 + i]);
   if (n <= p.budget) {                           // (the whole cluster)
     if (rank == 0 && tid == 0) p.count[unit] = 0;
-    for (int i = rank * kEvictThreads + tid; i < n; i += cs * kEvictThreads) {
-      if (w_out != w) w_out[i] = w[i];
-      if (pos_out != pos) pos_out[i] = pos[i];
-    }
     return;
-  }
-
-  const int share = (n + cs - 1) / cs;           // <= p.chunk
-  const int i0 = min(rank * share, n), mine = min(i0 + share, n) - i0;
-  for (int x = tid; x < 4 * 256; x += kEvictThreads) hist[x >> 8][x & 255] = 0;
-  const int last = __ldg(p.seen + b) - p.keep_last;
-  for (int i = tid; i < mine; i += kEvictThreads) {
-    const int at = pos[i0 + i];
-    keys[i] = at < p.keep_first || at >= last ? 0xffffffffu : weight_key(w[i0 + i]);
   }
   __syncthreads();
 
-  // ---- the budget-th largest key: eight bits a pass
-  uint32_t prefix = 0;
-  int need = p.budget;
+  // ---- the budget-th largest key
+  uint32_t prefix = 0, need = p.budget;
+  int shift = 32;
+  bool ties = true;                              // of the keys at the edge only the first `need` stay
 #pragma unroll 1
-  for (int pass = 0; pass < 4; ++pass) {
-    const int shift = 24 - 8 * pass;
+  for (int pass = 0; pass < 3; ++pass) {
+    const int above = shift, width = pass < 2 ? 11 : 10;
+    shift -= width;
+#pragma unroll 4
     for (int i = tid; i < mine; i += kEvictThreads) {
       const uint32_t key = keys[i];
-      if (pass == 0 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[pass][(key >> shift) & 255], 1u);
+      if (pass == 0 || key >> above == prefix) atomicAdd(&hist[pass][key >> shift & ((1u << width) - 1)], 1u);
     }
-    cluster.sync();
-    {
-      // two threads a bin, each half of the CTAs
-      const int bin = tid & 255, half = tid >> 8;
-      uint32_t s = 0;
-      for (int c = half; c < cs; c += 2) s += cluster.map_shared_rank(&hist[pass][0], c)[bin];
-      bins[half][bin] = s;
+    sync();
+    // thread t: bins 2047 - 2 t and the one below, so that the sums run from the top
+    uint32_t c0 = 0, c1 = 0;
+#pragma unroll
+    for (int c = 0; c < kEvictCluster; ++c) {
+      if (c >= cs) break;
+      const uint2 v = *reinterpret_cast<const uint2*>(
+          cluster.map_shared_rank(&hist[pass][0], c) + 2046 - 2 * tid);
+      c0 += v.y;
+      c1 += v.x;
     }
-    __syncthreads();
-    if (tid < 32) {                              // lane l: bins 255 - 8 l down to 248 - 8 l
-      int s = 0;
-      int c[8];
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const int bin = 255 - 8 * tid - x;
-        c[x] = static_cast<int>(bins[0][bin] + bins[1][bin]);
-        s += c[x];
-      }
-      int incl = s;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (tid >= o) incl += y;
-      }
-      int above = incl - s;
-#pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        if (above < need && need <= above + c[x]) {
-          found[0] = 255 - 8 * tid - x;
-          found[1] = need - above;
-        }
-        above += c[x];
-      }
+    uint32_t all;
+    const uint32_t before = block_scan(c0 + c1, sums, &all);
+    if (before < need && need <= before + c0 + c1) {
+      const bool second = need > before + c0;
+      found[0] = 2047 - 2 * tid - second;
+      found[1] = need - before - (second ? c0 : 0);
+      found[2] = second ? c1 : c0;
     }
     __syncthreads();
-    prefix = prefix << 8 | static_cast<uint32_t>(found[0]);
+    prefix = prefix << width | found[0];
     need = found[1];
+    if (need == found[2]) {                      // (the same in every CTA) all of them stay
+      ties = false;
+      break;
+    }
   }
-  // kept: keys above `prefix`, and the first `need` of those equal to it
+  // kept: keys whose bits from `shift` up are above `prefix`, or equal to it and, with ties
+  // (shift is 0 then), among the first `need`
 
-  // ---- ranks.  A thread owns `each` consecutive keys (an odd number: no bank conflicts)
-  const int each = ((mine + kEvictThreads - 1) / kEvictThreads) | 1;
-  const int a0 = min(tid * each, mine), a1 = min(a0 + each, mine);
-  int eq = 0;
-  for (int i = a0; i < a1; ++i) eq += keys[i] == prefix;
-  int all;
-  int eq_at = block_scan(eq, sums, &all);
-  if (tid == 0) counts[0] = all;
-  cluster.sync();
-  for (int c = 0; c < rank; ++c) eq_at += cluster.map_shared_rank(counts, c)[0];
-  int holes = 0, moved = 0, e = eq_at;
-  for (int i = a0; i < a1; ++i) {
-    const bool kept = keys[i] > prefix || (keys[i] == prefix && e++ < need);
-    if (i0 + i < p.budget) holes += !kept; else moved += kept;
-  }
-  int n_holes, n_moved;
-  int hole_at = block_scan(holes, sums, &n_holes);
-  int move_at = block_scan(moved, sums, &n_moved);
-  if (tid == 0) {
-    counts[1] = n_holes;
-    counts[2] = n_moved;
-  }
-  cluster.sync();
-  int total = 0;
-  for (int c = 0; c < cs; ++c) {
-    const int* other = cluster.map_shared_rank(counts, c);
-    if (c < rank) {
-      hole_at += other[1];
-      move_at += other[2];
+  // ---- ranks, by rounds of a key a thread: a warp's flags are one ballot, and the counts of
+  // (round, warp) are summed in the order of the keys
+  const int rounds = (p.chunk + kEvictThreads - 1) / kEvictThreads;   // <= 32
+  const uint32_t below_me = (1u << lane) - 1;
+  uint32_t all;
+  if (ties) {
+    for (int x = 0; x < rounds; ++x) {
+      const int i = x * kEvictThreads + tid;
+      const uint32_t eq = __ballot_sync(0xffffffffu, i < mine && keys[i] == prefix);
+      if (lane == 0) equals[x * 32 + warp] = __popc(eq);
     }
-    total += other[2];
+    __syncthreads();
+    uint32_t before = block_scan(tid < rounds * 32 ? equals[tid] : 0, sums, &all);
+    if (cs > 1) {
+      if (tid == 0) counts[0] = all;
+      cluster.sync();
+      for (int c = 0; c < rank; ++c) before += cluster.map_shared_rank(counts, c)[0];
+    }
+    if (tid < rounds * 32) equals[tid] = before;
+    __syncthreads();
   }
+  uint32_t free_place = 0, moved = 0;            // this round's ballots
+  auto flags = [&](int x) {
+    const int i = x * kEvictThreads + tid;
+    const bool live = i < mine;
+    const uint32_t key = live ? keys[i] : 0, top = key >> shift;
+    bool kept = top > prefix || top == prefix;
+    if (ties) {
+      const bool eq = live && key == prefix;
+      const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
+      if (eq) kept = equals[x * 32 + warp] + __popc(eqs & below_me) < need;
+    }
+    const bool low = i0 + i < p.budget;
+    free_place = __ballot_sync(0xffffffffu, live && low && !kept);
+    moved = __ballot_sync(0xffffffffu, live && !low && kept);
+  };
+  for (int x = 0; x < rounds; ++x) {
+    flags(x);
+    if (lane == 0) places[x * 32 + warp] = __popc(free_place) | __popc(moved) << 16;
+  }
+  __syncthreads();
+  uint32_t before = block_scan(tid < rounds * 32 ? places[tid] : 0, sums, &all);
+  int total = static_cast<int>(all >> 16), free_at = 0, move_at = 0;
+  if (cs > 1) {
+    if (tid == 0) counts[1] = all;
+    cluster.sync();
+    total = 0;
+#pragma unroll
+    for (int c = 0; c < kEvictCluster; ++c) {
+      if (c >= cs) break;
+      const uint32_t other = cluster.map_shared_rank(counts, c)[1];
+      if (c < rank) {
+        free_at += static_cast<int>(other & 0xffff);
+        move_at += static_cast<int>(other >> 16);
+      }
+      total += static_cast<int>(other >> 16);
+    }
+  }
+  if (tid < rounds * 32) places[tid] = before;
+  __syncthreads();
   int2* moves = p.moves + static_cast<long long>(unit) * p.move_rows;
-  e = eq_at;
-  for (int i = a0; i < a1; ++i) {
-    const int at = i0 + i;
-    const bool kept = keys[i] > prefix || (keys[i] == prefix && e++ < need);
-    if (at < p.budget) {
-      if (!kept) moves[hole_at++].x = at;
-    } else if (kept) {
-      moves[move_at++].y = at;
-    }
-  }
-  if (w_out != w || pos_out != pos) {
-    for (int i = tid; i < mine && i0 + i < p.budget; i += kEvictThreads) {
-      // (places about to be filled get their old values first; the moves below come after
-      // the barrier)
-      if (w_out != w) w_out[i0 + i] = w[i0 + i];
-      if (pos_out != pos) pos_out[i0 + i] = pos[i0 + i];
-    }
+  for (int x = 0; x < rounds; ++x) {
+    flags(x);
+    const uint32_t base = places[x * 32 + warp];
+    const int at = i0 + x * kEvictThreads + tid;
+    if (free_place >> lane & 1) moves[free_at + (base & 0xffff) + __popc(free_place & below_me)].x = at;
+    if (moved >> lane & 1) moves[move_at + (base >> 16) + __popc(moved & below_me)].y = at;
   }
   if (rank == 0 && tid == 0) p.count[unit] = total;
-  cluster.sync();                                // the list is complete; no CTA's counts are read any more
+  sync();                                        // the list is complete; no CTA's memory is read any more
   for (int i = rank * kEvictThreads + tid; i < total; i += cs * kEvictThreads) {
     const int2 mv = __ldcg(moves + i);
     w_out[mv.x] = w[mv.y];
     pos_out[mv.x] = pos[mv.y];
   }
   if (p.fused) {
-    const int width = p.row_bytes <= 128 ? 8 : 32;
-    const int per = kEvictThreads / width;
-    for (int i = rank * per + tid / width; i < total; i += cs * per)
-      move_row(p, b, h, __ldcg(moves + i), tid % width, width);
+    const int width = p.row_bytes <= 128 ? 8 : 32, per = kEvictThreads / width;
+    move_rows(p, b, h, moves, rank * per + tid / width, cs * per, total, tid % width, width);
   }
 }
 
@@ -277,10 +324,9 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const __grid_c
   const int unit = blockIdx.y, b = unit / p.kv_heads, h = unit - b * p.kv_heads;
   const int total = __ldcg(p.count + unit);
   const int2* moves = p.moves + static_cast<long long>(unit) * p.move_rows;
-  const int width = p.row_bytes <= 128 ? 8 : p.row_bytes <= 256 ? 16 : 32;
-  const int per = kMoveThreads / width;
-  for (int i = blockIdx.x * per + threadIdx.x / width; i < total; i += gridDim.x * per)
-    move_row(p, b, h, __ldcg(moves + i), threadIdx.x % width, width);
+  const int width = p.row_bytes <= 128 ? 8 : p.row_bytes <= 256 ? 16 : 32, per = kMoveThreads / width;
+  move_rows(p, b, h, moves, blockIdx.x * per + threadIdx.x / width, gridDim.x * per, total,
+            threadIdx.x % width, width);
 }
 
 struct AdvanceParams {
@@ -443,17 +489,22 @@ extern "C" int iq_kv_evict(const iq_evict_args* a, void* stream) {
   const long long spare = rows - a->budget;
   const long long most = spare < a->budget ? (spare > 0 ? spare : 0) : a->budget;
   p.fused = most <= kEvictFusedMoves;
-  // CTAs a cluster: about eight keys a thread and pass
+  // CTAs a cluster: eight keys a thread and pass where that many CTAs run at once (two an SM);
+  // 32768 rows x 8 heads: four CTAs 25.9 us, eight 27.2, two 32.4; 52283 rows x 56 heads, which
+  // eight each would make two waves: four 33, eight 62
   int cluster = 1;
-  while (cluster < kEvictCluster && rows > 4096LL * cluster) cluster *= 2;
+  while (cluster < kEvictCluster &&
+         (rows > static_cast<long long>(kEvictChunk) * cluster ||
+          (rows > 8LL * kEvictThreads * cluster && units * cluster <= n_sm)))
+    cluster *= 2;
   p.chunk = static_cast<int>((rows + cluster - 1) / cluster);
   const int rc = kv_launch(evict_kernel, p, dim3(static_cast<unsigned>(units * cluster)), kEvictThreads,
                            p.chunk * 4, cluster, stream, a->pdl != 0);
   if (rc != IQ_OK || p.fused) return rc;
-  // eight rows of work for every group of lanes, the whole chip at most
+  // four rows for every group of lanes, twice the chip's threads at most
   const int per = kMoveThreads / (p.row_bytes <= 128 ? 8 : p.row_bytes <= 256 ? 16 : 32);
   long long x = (most + 4 * per - 1) / (4 * per);
-  const long long cap = (n_sm * 8 + units - 1) / units;
+  const long long cap = (n_sm * 16 + units - 1) / units;
   if (x > cap) x = cap;
   return kv_launch(evict_move_kernel, p, dim3(static_cast<unsigned>(x), static_cast<unsigned>(units)),
                    kMoveThreads, 0, 1, stream, true);

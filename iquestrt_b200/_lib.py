@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 from . import _build
 
@@ -161,6 +162,17 @@ class AdvanceArgs(C.Structure):
     ]
 
 
+def packer(cls) -> struct.Struct:
+    """Packs values in the order of a structure's fields into its memory layout: one call
+    instead of an attribute access a field."""
+    codes = {C.c_void_p: "P", C.c_int64: "q", C.c_int: "i", C.c_float: "f", C.c_size_t: "N"}
+    packed = struct.Struct("@" + "".join(codes[kind] for _, kind in cls._fields_) + "0P")
+    assert packed.size == C.sizeof(cls)
+    return packed
+
+
+PACK_ATTN, PACK_EVICT, PACK_ADVANCE = (packer(c) for c in (AttnArgs, EvictArgs, AdvanceArgs))
+
 _LIB = None
 
 
@@ -190,14 +202,16 @@ def load() -> C.CDLL:
         lib.iq_tail.argtypes = [C.POINTER(TailArgs), C.c_void_p, C.c_int]
         for name, struct in (("iq_linear", LinearArgs), ("iq_linear_static", LinearArgs),
                              ("iq_qkv_heads", HeadsArgs), ("iq_router", RouterArgs),
-                             ("iq_moe_gate", MoeGateArgs), ("iq_moe_down", MoeDownArgs),
-                             ("iq_attn_decode", AttnArgs), ("iq_kv_evict", EvictArgs),
-                             ("iq_kv_advance", AdvanceArgs)):
+                             ("iq_moe_gate", MoeGateArgs), ("iq_moe_down", MoeDownArgs)):
             fn = getattr(lib, name)
             fn.restype = C.c_int
             fn.argtypes = [C.POINTER(struct), C.c_void_p]
         lib.iq_linear_static_status.restype = C.c_int
         lib.iq_linear_static_status.argtypes = [C.POINTER(C.c_int), C.c_void_p]
+        for name in ("iq_attn_decode", "iq_kv_evict", "iq_kv_advance"):
+            fn = getattr(lib, name)              # (a structure, or its packed bytes)
+            fn.restype = C.c_int
+            fn.argtypes = [C.c_void_p, C.c_void_p]
         lib.iq_attn_work_bytes.restype = C.c_size_t
         lib.iq_attn_work_bytes.argtypes = [C.c_int] * 7
         lib.iq_evict_work_bytes.restype = C.c_size_t

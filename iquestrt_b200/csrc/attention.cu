@@ -36,8 +36,6 @@
 
 #include <atomic>
 #include <type_traits>
-#include <mutex>
-#include <unordered_set>
 
 #include <cuda_fp16.h>
 
@@ -1229,39 +1227,38 @@ __global__ void __launch_bounds__(256) attn_weights_kernel(const __grid_constant
 
 // ------------------------------------------------------------------------------------
 // host side
-static std::mutex g_attn_mutex;
-
-static int attn_sms() {
-  static int per_device[64] = {};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  std::lock_guard<std::mutex> lock(g_attn_mutex);
-  if (per_device[dev] == 0) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    per_device[dev] = n;
+// SMs of the current device, and which it is; 0 where that fails.
+static int attn_sms(int* dev) {
+  static std::atomic<int> per_device[64];
+  if (cudaGetDevice(dev) != cudaSuccess || *dev < 0 || *dev >= 64) return 0;
+  int n = per_device[*dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, *dev) != cudaSuccess) return 0;
+    per_device[*dev].store(n, std::memory_order_relaxed);
   }
-  return per_device[dev];
+  return n;
 }
 
-static bool attn_smem_optin(const void* fn, int bytes) {
-  static std::unordered_set<uint64_t> done;
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return false;
-  const uint64_t key = (reinterpret_cast<uint64_t>(fn) << 6) ^ static_cast<uint64_t>(dev);
-  std::lock_guard<std::mutex> lock(g_attn_mutex);
-  if (done.count(key)) return true;
-  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+// Per kernel and device, once: the opt-in to its shared memory, and (where registers move
+// between its warps) that it was compiled for as many as they share.
+template <class K>
+static bool attn_ready(K kernel, std::atomic<uint64_t>& done, int dev, int smem, int regs) {
+  const uint64_t bit = uint64_t{1} << dev;       // dev < 64, see attn_sms
+  if (done.load(std::memory_order_acquire) & bit) return true;
+  if (regs > 0) {
+    cudaFuncAttributes at{};
+    if (cudaFuncGetAttributes(&at, kernel) != cudaSuccess || at.numRegs < regs) return false;
+  }
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return false;
-  done.insert(key);
+  done.fetch_or(bit, std::memory_order_release);
   return true;
 }
 
 template <class K, class... Args>
 static int attn_launch(K kernel, dim3 grid, int threads, int smem, void* stream, bool pdl,
                        const Args&... args) {
-  if (smem > 48 * 1024 && !attn_smem_optin(reinterpret_cast<const void*>(kernel), smem))
-    return IQ_ERR_CUDA;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
@@ -1374,7 +1371,7 @@ static int attn_map(CUtensorMap* out, const void* base, const AttnParams& p, lon
 }
 
 template <class G>
-static int attn_run(AttnParams& p, int n_sm, bool pdl, void* stream) {
+static int attn_run(AttnParams& p, int n_sm, int dev, bool pdl, void* stream) {
   const long long tiles = static_cast<long long>(p.batch) * (p.kv_heads / G::HG) * p.n_rb *
                           ((p.max_rows + G::TK - 1) / G::TK + 2);
   if (tiles > 0x7fffffffLL) return IQ_ERR_UNSUPPORTED;
@@ -1386,15 +1383,8 @@ static int attn_run(AttnParams& p, int n_sm, bool pdl, void* stream) {
   // (pages of 16 rows, 128k rows of e4m3: 54 us against 58; pages of one row need 64 a head).
   // Boxes leave less to do per tile where there are few (4096 rows: 8.9 us against 11.4).
   p.gather = 2 * G::BOXES * (G::KPW / box) * (G::HG / p.box_heads) * G::KG > 16;
-  if (G::MOVE_REGS) {                            // (a launch with fewer registers would wait for good)
-    static std::atomic<int> regs{0};
-    if (regs.load() == 0) {
-      cudaFuncAttributes at{};
-      if (cudaFuncGetAttributes(&at, attn_kernel<G>) != cudaSuccess) return IQ_ERR_CUDA;
-      regs.store(at.numRegs);
-    }
-    if (regs.load() < G::REGS) return IQ_ERR_CUDA;
-  }
+  static std::atomic<uint64_t> done{0};          // (a launch with fewer registers would wait for good)
+  if (!attn_ready(attn_kernel<G>, done, dev, G::SMEM, G::MOVE_REGS ? G::REGS : 0)) return IQ_ERR_CUDA;
   int rc = attn_map(&p.k_map, p.k, p, p.k_row, p.k_head, G::ELT, G::PITCH);
   if (rc == IQ_OK) rc = attn_map(&p.v_map, p.v, p, p.v_row, p.v_head, G::ELT, G::PITCH);
   if (rc != IQ_OK) return rc;
@@ -1414,30 +1404,30 @@ static int attn_run(AttnParams& p, int n_sm, bool pdl, void* stream) {
 // q in shared memory) left too few registers: 67 us against 37 for 32 rows over 32k keys of
 // e4m3, sixteen warps of eight rows 42.
 template <int KV, int DP, int HG>
-static int attn_pick_rows(AttnParams& p, int n_sm, bool pdl, void* stream) {
+static int attn_pick_rows(AttnParams& p, int n_sm, int dev, bool pdl, void* stream) {
   if constexpr (DP <= 128) {
-    if (p.rows_all <= 8) return attn_run<AttnGeo<KV, DP, 1, 1, HG, 8>>(p, n_sm, pdl, stream);
-    if (p.rows_all <= 16) return attn_run<AttnGeo<KV, DP, 2, 1, HG, 8>>(p, n_sm, pdl, stream);
-    if (p.rows_all <= 32) return attn_run<AttnGeo<KV, DP, 2, 2, HG, 8>>(p, n_sm, pdl, stream);
-    if constexpr (HG <= 2) return attn_run<AttnGeo<KV, DP, 2, 4, HG, 8>>(p, n_sm, pdl, stream);
+    if (p.rows_all <= 8) return attn_run<AttnGeo<KV, DP, 1, 1, HG, 8>>(p, n_sm, dev, pdl, stream);
+    if (p.rows_all <= 16) return attn_run<AttnGeo<KV, DP, 2, 1, HG, 8>>(p, n_sm, dev, pdl, stream);
+    if (p.rows_all <= 32) return attn_run<AttnGeo<KV, DP, 2, 2, HG, 8>>(p, n_sm, dev, pdl, stream);
+    if constexpr (HG <= 2) return attn_run<AttnGeo<KV, DP, 2, 4, HG, 8>>(p, n_sm, dev, pdl, stream);
   } else {
     constexpr int W = KV == IQ_ACT_BF16 ? 4 : 8;     // (two stages of eight rings do not fit)
-    if (p.rows_all <= 8) return attn_run<AttnGeo<KV, DP, 1, 1, HG, W>>(p, n_sm, pdl, stream);
-    if (p.rows_all <= 16) return attn_run<AttnGeo<KV, DP, 2, 1, HG, W>>(p, n_sm, pdl, stream);
+    if (p.rows_all <= 8) return attn_run<AttnGeo<KV, DP, 1, 1, HG, W>>(p, n_sm, dev, pdl, stream);
+    if (p.rows_all <= 16) return attn_run<AttnGeo<KV, DP, 2, 1, HG, W>>(p, n_sm, dev, pdl, stream);
     if constexpr (HG <= 2) {
-      if (p.rows_all <= 32) return attn_run<AttnGeo<KV, DP, 2, 2, HG, 8>>(p, n_sm, pdl, stream);
+      if (p.rows_all <= 32) return attn_run<AttnGeo<KV, DP, 2, 2, HG, 8>>(p, n_sm, dev, pdl, stream);
     }
-    if constexpr (HG == 1) return attn_run<AttnGeo<KV, DP, 2, 4, 1, 8>>(p, n_sm, pdl, stream);
+    if constexpr (HG == 1) return attn_run<AttnGeo<KV, DP, 2, 4, 1, 8>>(p, n_sm, dev, pdl, stream);
   }
   return IQ_ERR_UNSUPPORTED;
 }
 
 template <int KV, int DP>
-static int attn_pick(AttnParams& p, int n_sm, bool pdl, void* stream) {
+static int attn_pick(AttnParams& p, int n_sm, int dev, bool pdl, void* stream) {
   switch (head_group(p.kv_heads, block_rows(p.rows_all), p.dim)) {
-    case 4: return attn_pick_rows<KV, DP, 4>(p, n_sm, pdl, stream);
-    case 2: return attn_pick_rows<KV, DP, 2>(p, n_sm, pdl, stream);
-    default: return attn_pick_rows<KV, DP, 1>(p, n_sm, pdl, stream);
+    case 4: return attn_pick_rows<KV, DP, 4>(p, n_sm, dev, pdl, stream);
+    case 2: return attn_pick_rows<KV, DP, 2>(p, n_sm, dev, pdl, stream);
+    default: return attn_pick_rows<KV, DP, 1>(p, n_sm, dev, pdl, stream);
   }
 }
 
@@ -1482,7 +1472,8 @@ extern "C" int iq_attn_decode(const iq_attn_args* a, void* stream) {
   if (((reinterpret_cast<uint64_t>(a->q) | reinterpret_cast<uint64_t>(a->out)) & 15) ||
       ((a->q_b | a->q_r | a->q_h | a->o_b | a->o_r | a->o_h) & 7))
     return IQ_ERR_ARG;
-  const int n_sm = attn_sms();
+  int dev = 0;
+  const int n_sm = attn_sms(&dev);
   if (n_sm == 0 || n_sm > kAttnMaxCtas) return IQ_ERR_CUDA;
 
   AttnParams p{};
@@ -1533,16 +1524,16 @@ extern "C" int iq_attn_decode(const iq_attn_args* a, void* stream) {
   int rc;
   switch (pad_dim(a->head_dim, static_cast<int>(elt), a->page_size)) {
     case 64:
-      rc = bf16 ? attn_pick<IQ_ACT_BF16, 64>(p, n_sm, pdl, stream)
-                : attn_pick<IQ_ACT_E4M3, 64>(p, n_sm, pdl, stream);
+      rc = bf16 ? attn_pick<IQ_ACT_BF16, 64>(p, n_sm, dev, pdl, stream)
+                : attn_pick<IQ_ACT_E4M3, 64>(p, n_sm, dev, pdl, stream);
       break;
     case 128:
-      rc = bf16 ? attn_pick<IQ_ACT_BF16, 128>(p, n_sm, pdl, stream)
-                : attn_pick<IQ_ACT_E4M3, 128>(p, n_sm, pdl, stream);
+      rc = bf16 ? attn_pick<IQ_ACT_BF16, 128>(p, n_sm, dev, pdl, stream)
+                : attn_pick<IQ_ACT_E4M3, 128>(p, n_sm, dev, pdl, stream);
       break;
     default:
-      rc = bf16 ? attn_pick<IQ_ACT_BF16, 256>(p, n_sm, pdl, stream)
-                : attn_pick<IQ_ACT_E4M3, 256>(p, n_sm, pdl, stream);
+      rc = bf16 ? attn_pick<IQ_ACT_BF16, 256>(p, n_sm, dev, pdl, stream)
+                : attn_pick<IQ_ACT_E4M3, 256>(p, n_sm, dev, pdl, stream);
   }
   if (rc != IQ_OK || !weights) return rc;
   // enough blocks for four waves of the chip, never more than the rows need

@@ -391,65 +391,81 @@ def linear_static_status() -> int:
 
 
 # ---------------------------------------------------------------------- the paged KV cache
-def _gpu(name, t):
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor, got {t.device}")
+# These calls are a few microseconds of device time each, so their checks read every
+# tensor's properties once and the arguments are packed in one go.
+_BF16, _F32, _I32, _I64 = torch.bfloat16, torch.float32, torch.int32, torch.int64
 
 
-def _on(dev, name, args):
-    """Calls entry point `name` on `dev`'s current stream, with `dev` as the current device."""
+def _on(index, name, packed):
+    """Calls entry point `name` on device `index`'s current stream, with it as the current
+    device."""
     fn = getattr(_lib.load(), name)
-    if dev.index == torch.cuda.current_device():
-        _lib.check(name, fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream))
+    if index == torch._C._cuda_getDevice():
+        code = fn(packed, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            _lib.check(name, fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream))
+        with torch.cuda.device(index):
+            code = fn(packed, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        raise _lib.IqError(name, code)
 
 
-def _strided(name, t, dtype, shape, dev, written=False):
-    """Checks a tensor whose last axis is contiguous (others may have any stride, no two
-    elements at one address where it is `written`); returns its strides."""
+def _take(name, t, dtype, shape, index):
+    """Checks a tensor whose last axis is contiguous; returns its strides."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{name} must have dtype {dtype}, got {t.dtype}")
-    if t.device != dev:
-        raise ValueError(f"{name} must be on {dev}, got {t.device}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, the call's other tensors are on "
+                         f"{'cpu' if index < 0 else f'cuda:{index}'}")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     st = t.stride()
     if st[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{name} must be contiguous along its last axis")
-    if written and not t.is_contiguous():
+    return st
+
+
+def _take_out(name, t, dtype, shape, index):
+    """`_take` for a tensor that is written: no two elements at one address."""
+    st = _take(name, t, dtype, shape, index)
+    if not t.is_contiguous():
         reach = 1
         for size, step in sorted(zip(shape, st), key=lambda x: x[1]):
             if size > 1:
                 if step < reach:
                     raise ValueError(f"{name} must not overlap itself (strides {st})")
-                reach = step * (size - 1) + reach
+                reach += step * (size - 1)
     return st
 
 
-def _cache_pair(k_cache, v_cache, dev):
+def _cache_pair(k_cache, v_cache, index):
     if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 3:
         raise ValueError("the KV caches must be [capacity, kv_heads, head_dim] tensors")
-    if k_cache.dtype != torch.bfloat16 and k_cache.dtype != E4M3:
+    dtype, shape = k_cache.dtype, k_cache.shape
+    if dtype is not _BF16 and dtype is not E4M3:
         raise ValueError("the KV caches must both be bf16 or both e4m3")
-    ks = _strided("k_cache", k_cache, k_cache.dtype, k_cache.shape, dev, True)
-    vs = _strided("v_cache", v_cache, k_cache.dtype, k_cache.shape, dev, True)
-    return ks, vs
+    return (shape, ACT_E4M3 if dtype is E4M3 else ACT_BF16,
+            _take_out("k_cache", k_cache, dtype, shape, index),
+            _take_out("v_cache", v_cache, dtype, shape, index))
 
 
-def _paging(a, page_table, page_size, batch, dev):
-    st = _strided("page_table", page_table, torch.int32, page_table.shape, dev)
-    if page_table.dim() != 2 or page_table.shape[0] != batch or page_table.shape[1] < 1:
-        raise ValueError(f"page_table must be [{batch}, pages >= 1], got "
-                         f"{tuple(page_table.shape)}")
+def _pages(page_table, page_size, batch, index):
+    """(stride of the table's rows, pages a row); checks the table and the page size."""
+    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2:
+        raise ValueError("page_table must be a [batch, pages] tensor")
+    shape = page_table.shape
+    st = _take("page_table", page_table, _I32, shape, index)
+    if shape[0] != batch or shape[1] < 1:
+        raise ValueError(f"page_table must be [{batch}, pages >= 1], got {tuple(shape)}")
     if page_size < 1:
         raise ValueError(f"page_size must be at least 1, got {page_size}")
-    a.page_table, a.table_stride = page_table.data_ptr(), st[0]
-    a.page_size, a.max_pages = page_size, page_table.shape[1]
-    return page_size * page_table.shape[1]
+    return st[0], shape[1]
+
+
+def _gpu(name, index):
+    if index < 0:
+        raise ValueError(f"{name} must be a CUDA tensor")
 
 
 class AttnWork:
@@ -469,6 +485,7 @@ class AttnWork:
                 "512 query rows a key/value head)")
         self.buf = torch.empty(self.bytes, dtype=torch.uint8, device=device)
         self.ptr = self.buf.data_ptr()
+        self.index = self.buf.get_device()
 
 
 def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, scale=None,
@@ -488,61 +505,57 @@ def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, sca
     the query heads of its key/value head and the new tokens; the new tokens' own entries are
     set, and those of `positions` (int32, same shape) to the tokens' positions, `seen [batch]`
     (int32) being the tokens seen so far with the new ones.  Without `work` one is allocated
-    for the call.  A length or page out of range shows in `scratch`'s status word."""
+    for the call.  A length or page out of range shows in `scratch`'s status word.
+
+    Addresses of q, out and the caches, and their strides, are multiples of 16 bytes."""
     if not isinstance(q, torch.Tensor) or q.dim() != 4:
         raise ValueError("q must be a tensor [batch, q_len, q_heads, head_dim]")
-    dev, shape = q.device, q.shape
+    shape, index = q.shape, q.get_device()
     batch, q_len, q_heads, d = shape
-    a = _lib.AttnArgs()
-    qs = _strided("q", q, torch.bfloat16, shape, dev)
-    ks, vs = _cache_pair(k_cache, v_cache, dev)
-    capacity, kv_heads, kd = k_cache.shape
+    qs = _take("q", q, _BF16, shape, index)
+    (capacity, kv_heads, kd), kind, ks, vs = _cache_pair(k_cache, v_cache, index)
     if kd != d or kv_heads < 1 or q_heads % kv_heads:
         raise ValueError(f"q {tuple(shape)} does not fit caches of {kv_heads} heads of {kd}")
-    rows = _paging(a, page_table, page_size, batch, dev)
-    _strided("lengths", lengths, torch.int32, (batch,), dev)
+    ts, pages = _pages(page_table, page_size, batch, index)
+    _take("lengths", lengths, _I32, (batch,), index)
     if window < 0:
         raise ValueError(f"window must not be negative, got {window}")
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
-    os_ = _strided("out", out, torch.bfloat16, shape, dev, True)
+        out = torch.empty(shape, dtype=_BF16, device=q.device)
+    os_ = _take_out("out", out, _BF16, shape, index)
+    lse_ptr = w_ptr = pos_ptr = seen_ptr = w_rows = 0
+    ws = ps = (0, 0)
     if lse is not None:
-        _strided("lse", lse, torch.float32, shape[:3], dev)
+        _take("lse", lse, _F32, shape[:3], index)
         if not lse.is_contiguous():
             raise ValueError("lse must be contiguous")
-        a.lse = lse.data_ptr()
+        lse_ptr = lse.data_ptr()
     if weights is not None:
-        if weights.dim() != 3 or weights.shape[2] < rows:
-            raise ValueError(f"weights must be [{batch}, {kv_heads}, >= {rows}], got "
+        if weights.dim() != 3 or weights.shape[2] < page_size * pages:
+            raise ValueError(f"weights must be [{batch}, {kv_heads}, >= {page_size * pages}], got "
                              f"{tuple(weights.shape)}")
-        n = weights.shape[2]
-        ws = _strided("weights", weights, torch.float32, (batch, kv_heads, n), dev, True)
-        a.weights, a.w_b, a.w_h, a.weights_rows = weights.data_ptr(), ws[0], ws[1], n
+        w_rows = weights.shape[2]
+        ws = _take_out("weights", weights, _F32, (batch, kv_heads, w_rows), index)
+        w_ptr = weights.data_ptr()
     if (positions is None) != (seen is None) or (positions is not None and weights is None):
         raise ValueError("positions and seen come together, with weights")
     if positions is not None:
-        ps = _strided("positions", positions, torch.int32, weights.shape, dev, True)
-        _strided("seen", seen, torch.int32, (batch,), dev)
-        a.positions, a.p_b, a.p_h, a.seen = positions.data_ptr(), ps[0], ps[1], seen.data_ptr()
-    _gpu("q", q)
+        ps = _take_out("positions", positions, _I32, weights.shape, index)
+        _take("seen", seen, _I32, (batch,), index)
+        pos_ptr, seen_ptr = positions.data_ptr(), seen.data_ptr()
+    _gpu("q", index)
     if work is None:
         work = AttnWork(batch=batch, q_len=q_len, q_heads=q_heads, kv_heads=kv_heads, head_dim=d,
-                        rows=rows, weights=weights is not None, device=dev)
-    elif work.buf.device != dev:
-        raise ValueError(f"work must be on {dev}, got {work.buf.device}")
-    a.q, a.q_b, a.q_r, a.q_h = q.data_ptr(), qs[0], qs[1], qs[2]
-    a.k_cache, a.k_row, a.k_head = k_cache.data_ptr(), ks[0], ks[1]
-    a.v_cache, a.v_row, a.v_head = v_cache.data_ptr(), vs[0], vs[1]
-    a.kv_kind = ACT_E4M3 if k_cache.dtype == E4M3 else ACT_BF16
-    a.capacity, a.lengths = capacity, lengths.data_ptr()
-    a.batch, a.q_len, a.q_heads, a.kv_heads, a.head_dim = batch, q_len, q_heads, kv_heads, d
-    a.window, a.scale = window, d ** -0.5 if scale is None else scale
-    a.out, a.o_b, a.o_r, a.o_h = out.data_ptr(), os_[0], os_[1], os_[2]
-    a.work, a.work_bytes = work.ptr, work.bytes
-    if scratch is not None:
-        a.status = scratch.ptr
-    a.pdl = int(pdl)
-    _on(dev, "iq_attn_decode", a)
+                        rows=page_size * pages, weights=weights is not None, device=q.device)
+    elif work.index != index:
+        raise ValueError(f"work must be on cuda:{index}, got {work.buf.device}")
+    _on(index, "iq_attn_decode", _lib.PACK_ATTN.pack(
+        q.data_ptr(), qs[0], qs[1], qs[2], k_cache.data_ptr(), v_cache.data_ptr(),
+        ks[0], ks[1], vs[0], vs[1], kind, capacity, page_table.data_ptr(), ts, page_size, pages,
+        lengths.data_ptr(), batch, q_len, q_heads, kv_heads, d, window,
+        d ** -0.5 if scale is None else scale, out.data_ptr(), os_[0], os_[1], os_[2], lse_ptr,
+        w_ptr, ws[0], ws[1], w_rows, pos_ptr, ps[0], ps[1], seen_ptr, work.ptr, work.bytes,
+        0 if scratch is None else scratch.ptr, int(pdl)))
     return out
 
 
@@ -557,6 +570,7 @@ class EvictWork:
                              "rows (batch x heads up to 65535, rows up to 262144)")
         self.buf = torch.empty(self.bytes, dtype=torch.uint8, device=device)
         self.ptr = self.buf.data_ptr()
+        self.index = self.buf.get_device()
 
 
 def kv_evict(k_cache, v_cache, page_table, lengths, weights, positions, seen, *, page_size: int,
@@ -575,48 +589,40 @@ def kv_evict(k_cache, v_cache, page_table, lengths, weights, positions, seen, *,
     lengths.  Sequences must not share pages."""
     if not isinstance(weights, torch.Tensor) or weights.dim() != 3:
         raise ValueError("weights must be a tensor [batch, kv_heads, rows]")
-    dev = weights.device
-    batch, kv_heads, n = weights.shape
-    a = _lib.EvictArgs()
-    ks, vs = _cache_pair(k_cache, v_cache, dev)
-    capacity, kh, d = k_cache.shape
-    rows = _paging(a, page_table, page_size, batch, dev)
-    if kh != kv_heads or n < rows:
-        raise ValueError(f"weights must be [{batch}, {kh}, >= {rows}], got {tuple(weights.shape)}")
+    shape, index = weights.shape, weights.get_device()
+    batch, kv_heads, n = shape
+    (capacity, kh, d), kind, ks, vs = _cache_pair(k_cache, v_cache, index)
+    ts, pages = _pages(page_table, page_size, batch, index)
+    if kh != kv_heads or n < page_size * pages:
+        raise ValueError(f"weights must be [{batch}, {kh}, >= {page_size * pages}], got "
+                         f"{tuple(shape)}")
     if budget < 1 or keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget:
         raise ValueError(f"budget must be at least 1 and hold the protected rows, got {budget} for "
                          f"{keep_first} + {keep_last}")
     weights_out = weights if weights_out is None else weights_out
     positions_out = positions if positions_out is None else positions_out
-    ws = _strided("weights", weights, torch.float32, weights.shape, dev)
-    ps = _strided("positions", positions, torch.int32, weights.shape, dev)
-    wo = _strided("weights_out", weights_out, torch.float32, weights.shape, dev, True)
-    po = _strided("positions_out", positions_out, torch.int32, weights.shape, dev, True)
-    for name, t in (("lengths", lengths), ("seen", seen), ("lengths_out", lengths_out)):
-        _strided(name, t, torch.int32, (batch,), dev)
-    if lengths_out.data_ptr() == lengths.data_ptr():
+    ws = _take("weights", weights, _F32, shape, index)
+    ps = _take("positions", positions, _I32, shape, index)
+    wo = _take_out("weights_out", weights_out, _F32, shape, index)
+    po = _take_out("positions_out", positions_out, _I32, shape, index)
+    _take("lengths", lengths, _I32, (batch,), index)
+    _take("seen", seen, _I32, (batch,), index)
+    _take("lengths_out", lengths_out, _I32, (batch,), index)
+    n_ptr, out_ptr = lengths.data_ptr(), lengths_out.data_ptr()
+    if abs(out_ptr - n_ptr) < 4 * batch:
         raise ValueError("lengths_out must not be lengths")
-    _gpu("weights", weights)
+    _gpu("weights", index)
     if work is None:
-        work = EvictWork(batch=batch, kv_heads=kv_heads, rows=rows, device=dev)
-    elif work.buf.device != dev:
-        raise ValueError(f"work must be on {dev}, got {work.buf.device}")
-    a.k_cache, a.k_row, a.k_head = k_cache.data_ptr(), ks[0], ks[1]
-    a.v_cache, a.v_row, a.v_head = v_cache.data_ptr(), vs[0], vs[1]
-    a.kv_kind = ACT_E4M3 if k_cache.dtype == E4M3 else ACT_BF16
-    a.capacity, a.lengths, a.seen = capacity, lengths.data_ptr(), seen.data_ptr()
-    a.weights, a.w_b, a.w_h = weights.data_ptr(), ws[0], ws[1]
-    a.positions, a.p_b, a.p_h = positions.data_ptr(), ps[0], ps[1]
-    a.weights_out, a.wo_b, a.wo_h = weights_out.data_ptr(), wo[0], wo[1]
-    a.positions_out, a.po_b, a.po_h = positions_out.data_ptr(), po[0], po[1]
-    a.lengths_out = lengths_out.data_ptr()
-    a.batch, a.kv_heads, a.head_dim = batch, kv_heads, d
-    a.budget, a.keep_first, a.keep_last = budget, keep_first, keep_last
-    a.work, a.work_bytes = work.ptr, work.bytes
-    if scratch is not None:
-        a.status = scratch.ptr
-    a.pdl = int(pdl)
-    _on(dev, "iq_kv_evict", a)
+        work = EvictWork(batch=batch, kv_heads=kv_heads, rows=page_size * pages,
+                         device=weights.device)
+    elif work.index != index:
+        raise ValueError(f"work must be on cuda:{index}, got {work.buf.device}")
+    _on(index, "iq_kv_evict", _lib.PACK_EVICT.pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], vs[0], vs[1], kind, capacity,
+        page_table.data_ptr(), ts, page_size, pages, n_ptr, seen.data_ptr(), weights.data_ptr(),
+        ws[0], ws[1], positions.data_ptr(), ps[0], ps[1], weights_out.data_ptr(), wo[0], wo[1],
+        positions_out.data_ptr(), po[0], po[1], out_ptr, batch, kv_heads, d, budget, keep_first,
+        keep_last, work.ptr, work.bytes, 0 if scratch is None else scratch.ptr, int(pdl)))
     return lengths_out
 
 
@@ -631,26 +637,24 @@ def kv_advance(page_table, lengths, seen, slot, pos, *, page_size: int, capacity
     write, and stays as it was (with `scratch`'s status word set)."""
     if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:
         raise ValueError("lengths must be a tensor [batch]")
-    dev, batch = lengths.device, lengths.shape[0]
+    shape, index = lengths.shape, lengths.get_device()
+    batch = shape[0]
     if not 1 <= q_len <= 8:
         raise ValueError(f"q_len must be 1..8, got {q_len}")
     if batch < 1 or capacity < 1:
         raise ValueError("batch and capacity must be at least 1")
-    a = _lib.AdvanceArgs()
-    _paging(a, page_table, page_size, batch, dev)
+    ts, pages = _pages(page_table, page_size, batch, index)
     lengths_out = lengths if lengths_out is None else lengths_out
     seen_out = seen if seen_out is None else seen_out
-    for name, t in (("lengths", lengths), ("seen", seen), ("lengths_out", lengths_out),
-                    ("seen_out", seen_out)):
-        _strided(name, t, torch.int32, (batch,), dev)
-    for name, t in (("slot", slot), ("pos", pos)):
-        _strided(name, t, torch.int64, (batch * q_len,), dev)
-    _gpu("lengths", lengths)
-    a.capacity, a.lengths, a.seen = capacity, lengths.data_ptr(), seen.data_ptr()
-    a.lengths_out, a.seen_out = lengths_out.data_ptr(), seen_out.data_ptr()
-    a.slot, a.pos, a.batch, a.q_len = slot.data_ptr(), pos.data_ptr(), batch, q_len
-    if scratch is not None:
-        a.status = scratch.ptr
-    a.pdl = int(pdl)
-    _on(dev, "iq_kv_advance", a)
+    _take("lengths", lengths, _I32, shape, index)
+    _take("seen", seen, _I32, shape, index)
+    _take("lengths_out", lengths_out, _I32, shape, index)
+    _take("seen_out", seen_out, _I32, shape, index)
+    _take("slot", slot, _I64, (batch * q_len,), index)
+    _take("pos", pos, _I64, (batch * q_len,), index)
+    _gpu("lengths", index)
+    _on(index, "iq_kv_advance", _lib.PACK_ADVANCE.pack(
+        page_table.data_ptr(), ts, page_size, pages, capacity, lengths.data_ptr(), seen.data_ptr(),
+        lengths_out.data_ptr(), seen_out.data_ptr(), slot.data_ptr(), pos.data_ptr(), batch, q_len,
+        0 if scratch is None else scratch.ptr, int(pdl)))
     return slot, pos

@@ -397,8 +397,9 @@ int iq_kv_evict(const iq_evict_args* a, void* stream);
 /* The cache rows and positions of the next q_len tokens of every sequence: slot[b * q_len + r]
  * = the cache row of row lengths[b] + r (what iq_qkv_heads takes), pos[...] = seen[b] + r,
  * lengths_out = lengths + q_len, seen_out = seen + q_len (both may be the inputs themselves).
- * A sequence whose pages do not reach so far keeps its length and gets slots of -1, with
- * IQ_ERR_ROUTE in the status word. */
+ * A sequence whose pages do not reach so far, or whose positions would pass max_positions
+ * (0: no limit), keeps its length and gets slots of -1 and positions of 0, with IQ_ERR_ROUTE
+ * in the status word. */
 typedef struct iq_advance_args {
   const int* page_table;
   int64_t table_stride;
@@ -410,6 +411,7 @@ typedef struct iq_advance_args {
   int64_t* slot;
   int64_t* pos;
   int batch, q_len;
+  int max_positions;
   int* status;
   int pdl;
 } iq_advance_args;

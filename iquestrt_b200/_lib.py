@@ -158,7 +158,8 @@ class AdvanceArgs(C.Structure):
         ("page_size", C.c_int), ("max_pages", C.c_int), ("capacity", C.c_int),
         ("lengths", C.c_void_p), ("seen", C.c_void_p), ("lengths_out", C.c_void_p),
         ("seen_out", C.c_void_p), ("slot", C.c_void_p), ("pos", C.c_void_p),
-        ("batch", C.c_int), ("q_len", C.c_int), ("status", C.c_void_p), ("pdl", C.c_int),
+        ("batch", C.c_int), ("q_len", C.c_int), ("max_positions", C.c_int),
+        ("status", C.c_void_p), ("pdl", C.c_int),
     ]
 
 

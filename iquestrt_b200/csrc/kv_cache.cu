@@ -335,7 +335,7 @@ struct AdvanceParams {
   const int *lengths, *seen;
   int *lengths_out, *seen_out;
   long long *slot, *pos;
-  int batch, q_len;
+  int batch, q_len, max_positions;
   int* status;
 };
 
@@ -346,7 +346,8 @@ __global__ void __launch_bounds__(128) advance_kernel(const __grid_constant__ Ad
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b >= p.batch) return;
   const int n = p.lengths[b], seen = p.seen[b];
-  bool ok = n >= 0 && n <= p.max_rows - p.q_len;
+  bool ok = n >= 0 && n <= p.max_rows - p.q_len &&
+            (p.max_positions == 0 || (seen >= 0 && seen <= p.max_positions - p.q_len));
   int row[8];
 #pragma unroll
   for (int r = 0; r < 8; ++r) {
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(128) advance_kernel(const __grid_constant__ Ad
   for (int r = 0; r < 8; ++r) {
     if (r < p.q_len) {
       p.slot[b * p.q_len + r] = ok ? row[r] : -1;
-      p.pos[b * p.q_len + r] = seen + r;
+      p.pos[b * p.q_len + r] = ok ? seen + r : 0;
     }
   }
   p.lengths_out[b] = ok ? n + p.q_len : n;
@@ -515,7 +516,7 @@ extern "C" int iq_kv_advance(const iq_advance_args* a, void* stream) {
       !a->slot || !a->pos)
     return IQ_ERR_ARG;
   if (a->page_size < 1 || a->max_pages < 1 || a->capacity < 1 || a->batch < 1 || a->q_len < 1 ||
-      a->q_len > 8)
+      a->q_len > 8 || a->max_positions < 0)
     return IQ_ERR_ARG;
   const long long rows = static_cast<long long>(a->page_size) * a->max_pages;
   if (rows > 0x3fffffffLL || a->batch > (1 << 24)) return IQ_ERR_UNSUPPORTED;
@@ -526,7 +527,7 @@ extern "C" int iq_kv_advance(const iq_advance_args* a, void* stream) {
   p.lengths_out = a->lengths_out; p.seen_out = a->seen_out;
   p.slot = reinterpret_cast<long long*>(a->slot);
   p.pos = reinterpret_cast<long long*>(a->pos);
-  p.batch = a->batch; p.q_len = a->q_len;
+  p.batch = a->batch; p.q_len = a->q_len; p.max_positions = a->max_positions;
   p.status = a->status;
   return kv_launch(advance_kernel, p, dim3(static_cast<unsigned>((a->batch + 127) / 128)), 128, 0, 1,
                    stream, a->pdl != 0);

@@ -24,8 +24,8 @@ from __future__ import annotations
 import torch
 
 from . import ops
-from .kernels import (MoeDecodeKernels, MultimemARTail, MultimemMLPTail, OProjGemv,
-                      PrologueKernels, RouterSelect, TailKernels)
+from .kernels import (MoeDecodeKernels, MultimemARTail, MultimemMLPTail, OProjGemv, PagedAttention,
+                      PagedKvCache, PrologueKernels, RouterSelect, TailKernels)
 from .synth import HEADS, HeadShape, LayerShape, rope_tables
 from .workspace import Workspace
 
@@ -167,11 +167,16 @@ class DecodeSlice:
     """Consecutive decoder layers of one TP rank as one chain of launches: per layer the
     attention prologue (column-parallel QKV product, q/k norm, rotary embedding, KV-cache
     write), then the `DecodeLayer` (o_proj + attention tail, router, expert Gate, expert
-    Down + MLP tail).  The attention core between the two is not part of this library: the
-    layer's `ao` is a stand-in the caller supplies per layer, and the prologue's q and the
-    cache rows it writes are outputs nobody consumes here.  Everything else is chained as in
-    the model: layer i's output is layer i+1's residual, and its norm (under layer i+1's
-    attention norm) is what layer i+1's QKV product reads.
+    Down + MLP tail).  Layer i's output is layer i+1's residual, and its norm (under layer
+    i+1's attention norm) is what layer i+1's QKV product reads.
+
+    With `kv` (a `PagedKvCache` of as many layers; batch x q_len is the slice's `q_len`) the
+    attention runs between the two, over that cache (`window` > 0: sliding-window), the
+    step's rows, positions and rotary angles come from the cache's own counters
+    (`max_positions` bounds them), and sequences past the cache's budget are cut at the end
+    of the step: a captured step decodes the next token each time it is replayed.  Without
+    `kv` the attention output `ao` is a stand-in the caller supplies per layer, and the
+    prologue's q and the cache rows it writes are outputs nobody consumes here.
 
     `layers` is a list of `(lw, pw)`: `synth.make_layer` and `synth.make_prologue` dicts.  An
     even number of layers keeps the alternating all-reduce outputs in step with a captured
@@ -179,8 +184,18 @@ class DecodeSlice:
 
     def __init__(self, shape: LayerShape, layers, *, heads: HeadShape = HEADS, q_len: int = 1,
                  tp: int = 1, group=None, device="cuda", cache_rows: int = 4096,
-                 positions=None, **layer_kwargs):
+                 positions=None, kv: PagedKvCache | None = None, window: int = 0,
+                 max_positions: int = 1 << 17, **layer_kwargs):
         self.layers = list(layers)
+        self.kv = kv
+        if kv is not None:
+            qh, kh = heads.local(tp)
+            if (kv.batch * kv.q_len, kv.kv_heads, kv.head_dim) != (q_len, kh, heads.head_dim) \
+                    or len(kv.k) != len(self.layers):
+                raise ValueError(f"the KV cache must hold {len(self.layers)} layers of {kh} heads of "
+                                 f"{heads.head_dim} for {q_len} rows a step")
+            if positions is not None:
+                raise ValueError("with a KV cache the positions are the cache's")
         self.layer = DecodeLayer(shape, q_len=q_len, tp=tp, group=group, device=device,
                                  formats="benchmark", **layer_kwargs)
         qh, kh = heads.local(tp)
@@ -189,6 +204,14 @@ class DecodeSlice:
         self.prologue = PrologueKernels(shape.hidden, qh, kh, heads.head_dim, heads.rotary_dim,
                                         shape.eps, ws=self._ws, q_len=q_len,
                                         scratch=self.layer.scratch)
+        if kv is not None:
+            self.attention = PagedAttention(qh, kv, ws=self._ws, window=window)
+            self._ws.freeze()
+            self.k_cache, self.v_cache, self.slot = kv.k, kv.v, kv.slot
+            self._tables = rope_tables(range(max_positions), heads, device=device)
+            self.cos, self.sin = (torch.zeros(q_len, heads.rotary_dim, dtype=torch.bfloat16,
+                                              device=device) for _ in range(2))
+            return
         self._ws.freeze()
         if positions is None:
             positions = [32000 + r for r in range(q_len)]
@@ -208,21 +231,37 @@ class DecodeSlice:
                                           self.k_cache[i], self.v_cache[i], pdl=pdl)
         return q
 
-    def step(self, residual, xn, aos, *, pdl=True, visit=None):
+    def step(self, residual, xn, aos=None, *, pdl=True, visit=None):
         """One token step through every layer.  `residual`, `xn` `[q, hidden]` bf16: the
         stream entering layer 0 and its norm; `aos[i]` the stand-in attention output of
-        layer i (`[q, q_dim/tp]` bf16).  Returns the last layer's `(out, norm_out)`.
-        `visit(i, q, out, norm_out)` is called after each layer's launches are enqueued."""
+        layer i (`[q, q_dim/tp]` bf16; only without a KV cache).  Returns the last layer's
+        `(out, norm_out)`.  `visit(i, q, out, norm_out)` is called after each layer's
+        launches are enqueued."""
+        if (aos is None) == (self.kv is None):
+            raise ValueError("stand-in attention outputs are for a slice without a KV cache")
+        if self.kv is not None:
+            self.kv.advance(max_positions=self._tables[0].shape[0], pdl=pdl)
+            for table, rows in zip(self._tables, (self.cos, self.sin)):
+                torch.index_select(table, 0, self.kv.pos, out=rows)
         for i, (lw, _) in enumerate(self.layers):
             q = self.prologue_step(i, xn, pdl=pdl)
-            residual, xn = self.layer.step(aos[i], residual, lw, pdl=pdl)
+            ao = aos[i] if self.kv is None else self.attention(q, i, pdl=pdl)
+            residual, xn = self.layer.step(ao, residual, lw, pdl=pdl)
             if visit is not None:
                 visit(i, q, residual, xn)
+        if self.kv is not None and self.kv.budget is not None:
+            for i in range(len(self.layers)):
+                self.kv.evict(i, pdl=pdl)
         return residual, xn
 
     @property
     def launches_per_layer(self):
-        return 6
+        """Launches of one layer (with a budget: its eviction's selection among them; one more
+        where the rows above the budget are many).  The bookkeeping once a step is not
+        counted."""
+        if self.kv is None:
+            return 6
+        return 8 if self.kv.budget is None else 10
 
     def check(self) -> None:
         self.layer.check()
@@ -233,9 +272,10 @@ class HostSliceStep:
     the stream entering layer 0 and its norm from pinned host memory, every layer's
     launches, and the copy of the last layer's output back to pinned host memory (`HostStep`
     for the slice).  The stand-in attention outputs `aos` stay on the device, where an
-    attention kernel would have written them.  Captures the slice's CURRENT `layers`."""
+    attention kernel would have written them (None for a slice with a KV cache; building this
+    object then takes one step).  Captures the slice's CURRENT `layers`."""
 
-    def __init__(self, sl: DecodeSlice, aos, *, pdl: bool = True):
+    def __init__(self, sl: DecodeSlice, aos=None, *, pdl: bool = True):
         layer = sl.layer
         dev = layer.norm_out.device
         q, h = layer.q_len, layer.shape.hidden

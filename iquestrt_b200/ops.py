@@ -627,22 +627,23 @@ def kv_evict(k_cache, v_cache, page_table, lengths, weights, positions, seen, *,
 
 
 def kv_advance(page_table, lengths, seen, slot, pos, *, page_size: int, capacity: int,
-               q_len: int = 1, lengths_out=None, seen_out=None, scratch: Scratch | None = None,
-               pdl: bool = False):
+               q_len: int = 1, max_positions: int = 0, lengths_out=None, seen_out=None,
+               scratch: Scratch | None = None, pdl: bool = False):
     """The cache rows and positions of the next `q_len` tokens of every sequence
     (`iq_kv_advance`), on the device, so that a captured step finds its own rows: `slot` and
     `pos [batch * q_len]` (int64) are what `qkv_heads` and the rotary tables take.  `lengths`
     and `seen [batch]` (int32) grow by `q_len`, in place unless `lengths_out` / `seen_out` are
-    given.  A sequence whose pages end before gets slots of -1, which `qkv_heads` refuses to
-    write, and stays as it was (with `scratch`'s status word set)."""
+    given.  A sequence whose pages end before, or whose positions would reach `max_positions`
+    (the rows of a rotary table; 0: no limit), gets slots of -1, which `qkv_heads` refuses to
+    write, and positions of 0, and stays as it was (with `scratch`'s status word set)."""
     if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:
         raise ValueError("lengths must be a tensor [batch]")
     shape, index = lengths.shape, lengths.get_device()
     batch = shape[0]
     if not 1 <= q_len <= 8:
         raise ValueError(f"q_len must be 1..8, got {q_len}")
-    if batch < 1 or capacity < 1:
-        raise ValueError("batch and capacity must be at least 1")
+    if batch < 1 or capacity < 1 or max_positions < 0:
+        raise ValueError("batch and capacity must be at least 1, max_positions not negative")
     ts, pages = _pages(page_table, page_size, batch, index)
     lengths_out = lengths if lengths_out is None else lengths_out
     seen_out = seen if seen_out is None else seen_out
@@ -656,5 +657,5 @@ def kv_advance(page_table, lengths, seen, slot, pos, *, page_size: int, capacity
     _on(index, "iq_kv_advance", _lib.PACK_ADVANCE.pack(
         page_table.data_ptr(), ts, page_size, pages, capacity, lengths.data_ptr(), seen.data_ptr(),
         lengths_out.data_ptr(), seen_out.data_ptr(), slot.data_ptr(), pos.data_ptr(), batch, q_len,
-        0 if scratch is None else scratch.ptr, int(pdl)))
+        max_positions, 0 if scratch is None else scratch.ptr, int(pdl)))
     return slot, pos

@@ -355,6 +355,15 @@ def test_bad_pages_and_lengths_set_the_status(scratch):
                    scratch=scratch)
     assert scratch.status() == 5
     assert slot.tolist()[:2] == [-1, -1] and full_rows.tolist() == before.tolist()[:2] + [41]
+    assert pos.tolist() == [0, 0, 40]
+    # positions at the end of a rotary table
+    some = torch.tensor([3, 4, 5], dtype=torch.int32, device=DEV)
+    seen = torch.tensor([9, 10, 11], dtype=torch.int32, device=DEV)
+    ops.kv_advance(table, some, seen, slot, pos, page_size=16, capacity=k.shape[0],
+                   max_positions=11, scratch=scratch)
+    assert scratch.status() == 5
+    assert pos.tolist() == [9, 10, 0] and seen.tolist() == [10, 11, 11] and some.tolist() == [4, 5, 5]
+    assert slot.tolist()[2] == -1
 
 
 def test_captured_step_advances_by_itself(scratch):
@@ -492,3 +501,78 @@ def test_pages_of_any_size(scratch, kv, page):
             assert (got.float() - want.float()).abs().max() <= 2.0 ** -7 * want.float().abs().max()
         else:
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("budget", [None, 40])
+def test_decode_slice_over_a_paged_cache(budget):
+    """A slice whose attention reads the cache its prologue writes: each step's attention of
+    every layer against 64 bits on what the cache held, the layers' outputs bit for bit those
+    of a slice fed these attention outputs as stand-ins, and replays of the captured step bit
+    for bit the eager steps."""
+    from iquestrt_b200 import synth
+    from iquestrt_b200.kernels import PagedKvCache
+    from iquestrt_b200.layer import DecodeSlice
+    shape = synth.LayerShape(hidden=1024, q_dim=1024, n_experts=16, top_k=2, inter=256)
+    heads = synth.HeadShape(q_heads=8, kv_heads=2)
+    layers = [(synth.make_layer(shape, device=DEV, seed=9, layer=i),
+               synth.make_prologue(shape, heads, device=DEV, seed=9, layer=i)) for i in range(2)]
+
+    def make():
+        kv = PagedKvCache(2, 2, 2, 128, rows=64, page_size=16, budget=budget, keep_first=2,
+                          keep_last=10)
+        g = _gen(95)
+        for x in kv.k + kv.v:
+            x.copy_(torch.randn(x.shape, generator=g, device=DEV))
+        kv.set_lengths([33, 5])
+        return DecodeSlice(shape, layers, heads=heads, q_len=2, kv=kv, max_positions=200)
+
+    g = _gen(96)
+    inputs = [(torch.randn(2, 1024, generator=g, device=DEV).to(BF16),
+               torch.randn(2, 1024, generator=g, device=DEV).to(BF16)) for _ in range(12)]
+    sl, graphed = make(), make()
+    stand_in = DecodeSlice(shape, layers, heads=heads, q_len=2)
+    res, xn = (torch.empty_like(x) for x in inputs[0])
+    stream = torch.cuda.Stream()
+    warm = make()                           # every kernel's first launch, outside the capture
+    warm.step(*inputs[0])
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            replayed = graphed.step(res, xn)
+            replayed2 = graphed.step(res, xn)  # both all-reduce outputs' slots
+    torch.cuda.synchronize()
+    held = [33, 5]
+    for i in range(0, 12, 2):
+        eager = []
+        for s in (i, i + 1):
+            seen = []
+
+            def visit(layer, q, out, norm):
+                c = sl.kv
+                seen.append((q.clone(), sl.attention.out.clone(), c.k[layer].clone(),
+                             c.v[layer].clone(), c.lengths.clone(), out.clone(), norm.clone()))
+
+            sl.step(*inputs[i], visit=visit)
+            held = [n + 1 for n in held]
+            for q, ao, k, v, n, _, _ in seen:
+                assert n.tolist() == held
+                want = P.attn_decode(q.view(2, 1, 8, 128), k, v, sl.kv.page_table, n, 16)
+                _check(ao.view(2, 1, 8, 128), None, want, E4M3, 128, 64)
+            got = stand_in.step(*inputs[i], [x[1] for x in seen])
+            assert torch.equal(got[0], seen[-1][5]) and torch.equal(got[1], seen[-1][6])
+            eager.append(got[0].clone())
+            if budget is not None:
+                held = [min(n, budget) for n in held]
+            assert sl.kv.held.tolist() == held
+        res.copy_(inputs[i][0])
+        xn.copy_(inputs[i][1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(replayed2[0], eager[1])
+        for a, b in zip(sl.kv.k + sl.kv.v, graphed.kv.k + graphed.kv.v):
+            assert torch.equal(_bits(a), _bits(b))
+        assert graphed.kv.seen.tolist() == [33 + i + 2, 5 + i + 2]
+    sl.check()
+    graphed.check()
+    assert sl.kv.scratch.status() == 0

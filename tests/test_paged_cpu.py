@@ -100,7 +100,7 @@ def test_eviction_refuses(field, value, code):
 @pytest.mark.parametrize("field,value", [
     ("page_table", None), ("lengths", None), ("seen", None), ("lengths_out", None),
     ("seen_out", None), ("slot", None), ("pos", None), ("page_size", 0), ("max_pages", 0),
-    ("capacity", 0), ("batch", 0), ("q_len", 0), ("q_len", 9),
+    ("capacity", 0), ("batch", 0), ("q_len", 0), ("q_len", 9), ("max_positions", -1),
 ])
 def test_advance_refuses(field, value):
     L, lib = _lib()
@@ -220,3 +220,26 @@ def test_oracle_eviction_by_hand():
     assert out[1][:3, 0, 0].tolist() == [10.0, 11.0, 14.0]
     assert out[2][0, 0, :3].tolist() == [0.0, 2.0, 0.5] and out[3][0, 0, :3].tolist() == [0, 3, 9]
     assert out[4].tolist() == [3]
+
+
+def test_holders_refuse():
+    from iquestrt_b200.kernels import PagedAttention, PagedKvCache
+    from iquestrt_b200.workspace import Workspace
+    ok = dict(rows=64, page_size=16, device="cpu")
+    for change, message in ((dict(q_len=9), "q_len"), (dict(dtype=torch.float16), "bf16 or e4m3"),
+                            (dict(budget=64), "budget"), (dict(budget=0), "budget"),
+                            (dict(page_table=torch.zeros(2, 4)), "capacity")):
+        with pytest.raises(ValueError, match=message):
+            PagedKvCache(1, 2, 2, 128, **{**ok, **change})
+    kv = PagedKvCache(1, 2, 2, 128, **ok)
+    assert kv.capacity == 128 and kv.page_table.tolist() == [[0, 1, 2, 3], [4, 5, 6, 7]]
+    for lengths in ([1], [1, 65], [-1, 0]):
+        with pytest.raises(ValueError, match="lengths"):
+            kv.set_lengths(lengths)
+    kv.set_lengths([3, 64])
+    assert kv.held.tolist() == kv.seen.tolist() == [3, 64]
+    ws = Workspace(device="cpu")
+    with pytest.raises(ValueError, match="share"):
+        PagedAttention(3, kv, ws=ws)
+    with pytest.raises(ValueError, match="window"):
+        PagedAttention(4, kv, ws=ws, window=-1)

@@ -71,6 +71,7 @@ struct AttnParams {
   int* positions;
   long long p_b, p_h;
   const int* seen;
+  unsigned joins, weight_chunks;                 // blocks that join; blocks a (sequence, head)'s weights take
   int* status;
   int batch, q_len, q_heads, kv_heads, group, dim, window;
   int rows_all;                                  // group * q_len
@@ -418,8 +419,9 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
     ld.start(p, prefix, lens, per, i0);
     if (p.gather) {
       // Pages too small for boxes: thread t copies piece t % CPR of every (128 / CPR)-th row,
-      // for all heads of the unit; a page lookup a row.  Arrives at `full` when its copies have.
+      // for all heads of the unit.  Arrives at `full` when its copies have.
       constexpr int CPR = G::DPB / 16, ROWS = kCopyThreads / CPR, PIECES = G::PITCH / 16;
+      static_assert((G::KPW < 32 ? G::KPW : 32) % ROWS == 0, "whole passes");
       const int ct = tid - G::CONSUMERS, c = ct % CPR;
       const bool in_row = c * 16 < p.dim * G::ELT;
       int stage = 0;
@@ -434,27 +436,34 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
             break;
           }
           const uint32_t to = smem_u32(ring) + (kgr * G::STAGES + stage) * G::STAGE + c / PIECES * G::BOX;
-#pragma unroll 2
-          for (int r = ct / CPR; r < G::KPW; r += ROWS) {
-            const int j = ld.j + kgr * G::KPW + r;
-            int row = -1;
-            if (j >= ld.lo && j < ld.n) {
-              row = cache_row(p.pages, ld.b, j);
-              if (row < 0 && p.status) atomicCAS(p.status, 0, IQ_ERR_ROUTE);
+          const uint8_t* k0 = p.k + ld.h0 * p.k_head + c * 16;
+          const uint8_t* v0 = p.v + ld.h0 * p.v_head + c * 16;
+#pragma unroll 1
+          for (int base = 0; base < G::KPW; base += 32) {
+            // a lane looks up one row of thirty-two
+            const int j = ld.j + kgr * G::KPW + base + lane;
+            int mine = -1;
+            if (j >= ld.lo && j < ld.n && base + lane < G::KPW) {
+              mine = cache_row(p.pages, ld.b, j);
+              if (mine < 0 && p.status) atomicCAS(p.status, 0, IQ_ERR_ROUTE);
             }
-            const bool ok = row >= 0 && in_row;  // else zeros, and nothing is read
-            const long long at = ok ? row : 0;
-            const int piece = ok ? c * 16 : 0;
-            const uint8_t* k = p.k + at * p.k_row + ld.h0 * p.k_head + piece;
-            const uint8_t* v = p.v + at * p.v_row + ld.h0 * p.v_head + piece;
-            uint32_t dst = to + swizzled<G>(r, c % PIECES);
 #pragma unroll
-            for (int hd = 0; hd < G::HG; ++hd) {
-              cp_async16(dst, k, ok);
-              cp_async16(dst + G::HALF, v, ok);
-              dst += G::HEAD;
-              k += p.k_head;
-              v += p.v_head;
+            for (int pass = 0; pass < (G::KPW < 32 ? G::KPW : 32) / ROWS; ++pass) {
+              const int r = ct / CPR + pass * ROWS;
+              const int row = __shfl_sync(0xffffffffu, mine, r);
+              const bool ok = row >= 0 && in_row;  // else zeros, and nothing is read
+              const uint8_t* k = ok ? k0 + row * p.k_row : p.k;
+              const uint8_t* v = ok ? v0 + row * p.v_row : p.v;
+              const long long k_step = ok ? p.k_head : 0, v_step = ok ? p.v_head : 0;
+              uint32_t dst = to + swizzled<G>(base + r, c % PIECES);
+#pragma unroll
+              for (int hd = 0; hd < G::HG; ++hd) {
+                cp_async16(dst, k, ok);
+                cp_async16(dst + G::HALF, v, ok);
+                dst += G::HEAD;
+                k += k_step;
+                v += v_step;
+              }
             }
           }
           asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(
@@ -538,18 +547,24 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
   uint64_t* full = bar_full + kg * G::MAX_STAGES;
   uint64_t* free_ = bar_free + kg * G::MAX_STAGES;
 
-  // ---- rows of empty sequences
+  // ---- rows of empty sequences: some CTAs a sequence, 16 bytes a store
+  {
+    const int team = max(1, static_cast<int>(gridDim.x) / p.batch);
 #pragma unroll 1
-  for (int b = cta; b < p.batch; b += gridDim.x) {
-    if (prefix[b + 1] != prefix[b]) continue;
-    for (int u = tid; u < per; u += G::CONSUMERS) p.units[b * per + u] = make_int2(0, 0);
-    for (int i = tid; i < p.q_len * p.q_heads * p.dim; i += G::CONSUMERS) {
-      const int d = i % p.dim, head = i / p.dim % p.q_heads, tok = i / p.dim / p.q_heads;
-      p.out[b * p.o_b + tok * p.o_r + head * p.o_h + d] = __float2bfloat16_rn(0.f);
-      if (d == 0) {
-        const long long o = (static_cast<long long>(b) * p.q_len + tok) * p.q_heads + head;
-        if (p.lse) p.lse[o] = -INFINITY;
-        if (p.lse2) p.lse2[o] = -INFINITY;
+    for (int b = cta / team; b < p.batch; b += (gridDim.x + team - 1) / team) {
+      if (prefix[b + 1] != prefix[b]) continue;
+      for (int u = tid; u < per; u += G::CONSUMERS) p.units[b * per + u] = make_int2(0, 0);
+      const int pieces = p.dim / 8, heads = p.q_len * p.q_heads;
+#pragma unroll 1
+      for (int i = cta % team * G::CONSUMERS + tid; i < heads * pieces; i += team * G::CONSUMERS) {
+        const int th = i / pieces, d = i - th * pieces, tok = th / p.q_heads, head = th - tok * p.q_heads;
+        *reinterpret_cast<uint4*>(p.out + b * p.o_b + tok * p.o_r + head * p.o_h + d * 8) =
+            make_uint4(0, 0, 0, 0);
+        if (d == 0) {
+          const long long o = static_cast<long long>(b) * heads + th;
+          if (p.lse) p.lse[o] = -INFINITY;
+          if (p.lse2) p.lse2[o] = -INFINITY;
+        }
       }
     }
   }
@@ -564,6 +579,7 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
   // m: the reference the weights are relative to; mu: the same, 0 while there is none; thr:
   // how far above it a score may lie before the reference moves
   float m[G::NBW][2], mu[G::NBW][2], thr[G::NBW][2], l[G::NBW][2], acc[G::NBW][G::MT][4];
+  int last_key[G::NBW][2];
 
   // The reference only has to keep the weights inside their type's range, so it follows the
   // maximum lazily: it moves when a score lies more than kLimit above it, to kShift below
@@ -602,11 +618,17 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
       if (from_start && tid == 0) p.units[it.b * per + it.hb].x = cta;
 #pragma unroll
       for (int nb = 0; nb < G::NBW; ++nb) {
+        // the last key each of this lane's two columns sees
+        const int rc = r0 + (wr * G::NBW + nb) * 8 + 2 * t;
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          last_key[nb][y] = it.n - p.q_len + (p.q_len == 1 ? 0 : min((rc + y) / p.group, p.q_len - 1));
+      }
+      auto load_q = [&](int nb, uint32_t(&qr)[G::QREG]) {
         const int r = r0 + (wr * G::NBW + nb) * 8 + g;
         const bool live = r < p.rows_all;
-        const int tok = live ? r / p.group : 0, head = h * p.group + (live ? r - tok * p.group : 0);
+        const int tok = live && p.q_len > 1 ? r / p.group : 0, head = h * p.group + (live ? r - tok * p.group : 0);
         const __nv_bfloat16* src = p.q + it.b * p.q_b + tok * p.q_r + head * p.q_h;
-        uint32_t(&qr)[G::QREG] = qf[G::QS ? 0 : nb];
         if (G::KV == IQ_ACT_BF16) {
           // fragment order of the MMA: registers 2i, 2i+1 are channels 16i + 2t, 16i + 8 + 2t
 #pragma unroll
@@ -614,12 +636,8 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
             const int d = x * 8 + 2 * t;
             qr[x] = live && d < p.dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
           }
-          xs[nb][0] = xs[nb][1] = p.scale_log2;
         } else {
-          // lane t holds channels 64 k + 16 t .. + 15; bf16 values scaled by a power of two
-          // so that the row's largest lies in [1, 2): exact in half precision but for
-          // values 2^-14 below the row's largest
-          float big = 0.f;
+          // lane t holds channels 64 k + 16 t .. + 15
 #pragma unroll
           for (int x = 0; x < G::QREG; x += 4) {
             const int d = (x / 8) * 64 + t * 16 + (x % 8) * 2;
@@ -627,6 +645,21 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
             if (live && d < p.dim) w = *reinterpret_cast<const uint4*>(src + d);
             qr[x] = w.x; qr[x + 1] = w.y; qr[x + 2] = w.z; qr[x + 3] = w.w;
           }
+        }
+      };
+      if (!G::QS)
+#pragma unroll
+        for (int nb = 0; nb < G::NBW; ++nb) load_q(nb, qf[G::QS ? 0 : nb]);
+#pragma unroll
+      for (int nb = 0; nb < G::NBW; ++nb) {
+        uint32_t(&qr)[G::QREG] = qf[G::QS ? 0 : nb];
+        if (G::QS) load_q(nb, qr);
+        if (G::KV == IQ_ACT_BF16) {
+          xs[nb][0] = xs[nb][1] = p.scale_log2;
+        } else {
+          // bf16 values scaled by a power of two so that the row's largest lies in [1, 2):
+          // exact in half precision but for values 2^-14 below the row's largest
+          float big = 0.f;
 #pragma unroll
           for (int x = 0; x < G::QREG; ++x)
             big = fmaxf(big, fmaxf(fabsf(__uint_as_float(qr[x] << 16)),
@@ -675,30 +708,35 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
     }
     if (partial) {
       // values outside the unit: zeros; values that only some rows see: finite ones stay
+      constexpr int PIECES = G::PITCH / 16;
 #pragma unroll 1
-      for (int x = gtid; x < G::KPW * G::DPB / 16; x += GT) {
-        const int j = j0 + (x / (G::PITCH / 16)) % G::KPW;
+      for (int x = gtid; x < G::KPW * PIECES; x += GT) {
+        const int j = j0 + x / PIECES;
         if (j >= lo_all && j < hi_all) continue;
-        const uint32_t at = sv + x / (G::HEAD / 16) * G::BOX + x % (G::HEAD / 16) * 16;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (j >= it.lo && j < it.n) {
-          w = lds128(at);
-          if (!strip<G::KV>(w)) continue;
-          *not_finite = 1;
+#pragma unroll
+        for (int box = 0; box < G::BOXES; ++box) {
+          const uint32_t at = sv + box * G::BOX + x * 16;
+          uint4 w = make_uint4(0, 0, 0, 0);
+          if (j >= it.lo && j < it.n) {
+            w = lds128(at);
+            if (!strip<G::KV>(w)) continue;
+            *not_finite = 1;
+          }
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w.x), "r"(w.y),
+                       "r"(w.z), "r"(w.w)
+                       : "memory");
         }
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w.x),
-                     "r"(w.y), "r"(w.z), "r"(w.w)
-                     : "memory");
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       if (G::WR == 1) __syncwarp();
       else named_bar_sync(2 + warp / G::WR, GT);
     }
 
-    // The tiles of sixteen keys, SUBI at a time.  EDGE: some row does not see some key, or the
-    // scores are kept; the other form, nearly all tiles', has no branch but the reference's.
-    auto tiles = [&](auto edge) {
-      constexpr bool EDGE = decltype(edge)::value;
+    // The tiles of sixteen keys, SUBI at a time.  EDGE: some row does not see some key; SCORES:
+    // the scores may be kept.  With neither, nearly all tiles', there is no branch but the
+    // reference's.
+    auto tiles = [&](auto edge, auto keep) {
+      constexpr bool EDGE = decltype(edge)::value, SCORES = decltype(keep)::value;
 #pragma unroll 1
       for (int s0 = 0; s0 < G::SUB; s0 += G::SUBI) {
         if (EDGE && (j0 + s0 * 16 >= it.n || j0 + (s0 + G::SUBI) * 16 <= it.lo)) continue;
@@ -763,21 +801,19 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
         float x[G::NBW][G::SUBI][4];
         auto masked = [&](int nb) {              // -infinity for what this lane's rows do not see
           if (!EDGE) return;
-          const int r = r0 + (wr * G::NBW + nb) * 8 + 2 * t;
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            const int pos = it.n - p.q_len + min((r + y) / p.group, p.q_len - 1);
-            const int from = p.window ? max(0, pos - p.window + 1) : 0;
+            const int to = last_key[nb][y], from = p.window ? to - p.window : -1;
 #pragma unroll
             for (int sub = 0; sub < G::SUBI; ++sub)
 #pragma unroll
               for (int z = 0; z < 2; ++z) {
                 const int key = jt + sub * 16 + z * 8;
-                if (key < from || key > pos) x[nb][sub][2 * z + y] = -INFINITY;
+                if (key <= from || key > to) x[nb][sub][2 * z + y] = -INFINITY;
               }
           }
         };
-        if (EDGE && p.scores) {
+        if (SCORES && (!EDGE || p.scores)) {
 #pragma unroll
           for (int nb = 0; nb < G::NBW; ++nb) {
             const int r = r0 + (wr * G::NBW + nb) * 8 + 2 * t;
@@ -786,7 +822,7 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
             for (int sub = 0; sub < G::SUBI; ++sub)
 #pragma unroll
               for (int y = 0; y < 4; ++y) x[nb][sub][y] = sc[sub][nb][y] * xs[nb][y & 1];
-            if (partial) masked(nb);
+            masked(nb);
 #pragma unroll
             for (int sub = 0; sub < G::SUBI; ++sub) {
               const int j = jt + sub * 16;
@@ -794,8 +830,8 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
                            ((static_cast<long long>(it.b) * p.kv_heads + h) * p.score_rows + j) *
                                p.rows_pad + r;
               const float(&z)[4] = x[nb][sub];
-              if (j >= it.lo && j < it.n) *reinterpret_cast<float2*>(dst) = make_float2(z[0], z[1]);
-              if (j + 8 >= it.lo && j + 8 < it.n)
+              if (!EDGE || (j >= it.lo && j < it.n)) *reinterpret_cast<float2*>(dst) = make_float2(z[0], z[1]);
+              if (!EDGE || (j + 8 >= it.lo && j + 8 < it.n))
                 *reinterpret_cast<float2*>(dst + 8 * p.rows_pad) = make_float2(z[2], z[3]);
             }
           }
@@ -808,7 +844,7 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
 #pragma unroll
             for (int y = 0; y < 4; ++y)
               x[nb][sub][y] = fmaf(sc[sub][nb][y], xs[nb][y & 1], -mu[nb][y & 1]);
-          if (EDGE && partial) masked(nb);
+          masked(nb);
         };
 #pragma unroll
         for (int nb = 0; nb < G::NBW; ++nb) {
@@ -919,8 +955,12 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
         }
       }
     };
-    if (!partial && !p.scores) tiles(std::false_type{});
-    else if (j0 < it.n && j0 + G::KPW > it.lo) tiles(std::true_type{});
+    if (!partial) {
+      if (p.scores) tiles(std::false_type{}, std::true_type{});
+      else tiles(std::false_type{}, std::false_type{});
+    } else if (j0 < it.n && j0 + G::KPW > it.lo) {
+      tiles(std::true_type{}, std::true_type{});
+    }
 
     // the stage is free: one arrival a warp that reads it
     __syncwarp();
@@ -939,6 +979,7 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], o);
+        if constexpr (G::KG > 1)
 #pragma unroll 1
         for (int half = G::KG / 2; half >= 1; half >>= 1) {
           float* mine = join + ((((kg & (half - 1)) * G::HG + hg) * G::WR + wr) * G::NREG) * 32 + 4 * lane;
@@ -1075,6 +1116,89 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
 constexpr int kJoinThreads = 256;
 constexpr int kJoinParts = 160;                  // partial results of a unit, at most (one a CTA)
 
+// weights[b, h, j] += sum over the head's query rows of 2^(x_j - lse2): a thread a key, on the
+// scores the split kernel left behind (L2 holds most of them).  Each block works out the rows'
+// lse2 from the partial results for itself, so these blocks need not wait for those that join.
+// The step's own rows are set, not added to, and get their positions.
+constexpr int kWeightKeys = 1024;                // keys a block
+
+template <class G>
+__device__ __forceinline__ void add_weights(const AttnParams& p, int chunk, int bh, float* z /* [512] */) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int b = bh / p.kv_heads, h = bh - b * p.kv_heads;
+  const SeqSpan s = seq_span(clamp_length(p, b, false), p.q_len, p.window);
+  const int from = max(s.lo, chunk * kWeightKeys), to = min(s.n, (chunk + 1) * kWeightKeys);
+  if (from >= to) return;
+  for (int r = warp; r < p.rows_pad; r += kJoinThreads / 32) {
+    float v = INFINITY;                          // a padded or empty row adds nothing
+    if (r < p.rows_all) {
+      const int rb = r / G::RB;
+      const int2 c = __ldcg(p.units + (static_cast<long long>(b) * (p.kv_heads / G::HG) + h / G::HG) * p.n_rb + rb);
+      const int n = c.y - c.x + 1;
+      if (n <= 1) {
+        const int tok = r / p.group, head = h * p.group + r - tok * p.group;
+        v = __ldcg(p.lse2 + (static_cast<long long>(b) * p.q_len + tok) * p.q_heads + head);
+      } else {
+        float2 ml[kJoinParts / 32];
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kJoinParts / 32; ++i) {
+          const int k = lane + 32 * i;
+          ml[i] = make_float2(-INFINITY, 0.f);
+          if (k < n)
+            ml[i] = __ldcg(p.part_ml + (static_cast<size_t>(2 * (c.x + k) + (k == 0 ? 1 : 0)) * G::HG + h % G::HG) *
+                                           G::RB + r % G::RB);
+          top = fmaxf(top, ml[i].x);
+        }
+        top = warp_max(top);
+        const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int i = 0; i < kJoinParts / 32; ++i) sum += ex2(ml[i].x - base) * ml[i].y;
+        sum = warp_sum(sum);
+        v = sum > 0.f ? top + log2f(sum) : (sum == 0.f ? -INFINITY : sum);
+      }
+      if (v == -INFINITY) v = INFINITY;
+    }
+    if (lane == 0) z[r] = v;
+  }
+  __syncthreads();
+  // a thread's four keys are all in flight
+  constexpr int EACH = kWeightKeys / kJoinThreads;
+  const long long row = static_cast<long long>(b) * p.kv_heads + h;
+  float w[EACH], old[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int j = chunk * kWeightKeys + tid + i * kJoinThreads;
+    w[i] = old[i] = 0.f;
+    if (j >= from && j < to && j < s.n - p.q_len) old[i] = p.weights[b * p.w_b + h * p.w_h + j];
+  }
+#pragma unroll 2
+  for (int r = 0; r < p.rows_pad; r += 4) {
+    float4 x[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int j = chunk * kWeightKeys + tid + i * kJoinThreads;
+      if (j >= from && j < to)
+        x[i] = __ldcg(reinterpret_cast<const float4*>(p.scores + (row * p.score_rows + j) * p.rows_pad + r));
+    }
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const float zr = z[r + y];
+      if (zr == INFINITY) continue;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) w[i] += ex2((y == 0 ? x[i].x : y == 1 ? x[i].y : y == 2 ? x[i].z : x[i].w) - zr);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const int j = chunk * kWeightKeys + tid + i * kJoinThreads;
+    if (j < from || j >= to) continue;
+    p.weights[b * p.w_b + h * p.w_h + j] = old[i] + w[i];
+    if (j >= s.n - p.q_len && p.positions)
+      p.positions[b * p.p_b + h * p.p_h + j] = __ldg(p.seen + b) - s.n + j;
+  }
+}
+
 template <class G, bool WIDE>
 __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_constant__ AttnParams p) {
   __shared__ float fac[8][kJoinParts];
@@ -1085,11 +1209,17 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   const int per = p.kv_heads / G::HG * p.n_rb;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (blockIdx.x >= p.joins) {
+    if (blockIdx.y == 0 && blockIdx.z == 0)
+      add_weights<G>(p, (blockIdx.x - p.joins) % p.weight_chunks, (blockIdx.x - p.joins) / p.weight_chunks,
+                     reinterpret_cast<float*>(red));
+    return;
+  }
   const int u = blockIdx.x / G::HG, hg = blockIdx.x % G::HG;
   const int b = u / per, hb = u - b * per, h = hb / p.n_rb * G::HG + hg;
   const int block = blockIdx.y, r0 = hb % p.n_rb * G::RB + block * 8;
-  pdl_wait();
-  pdl_launch_dependents();
   const int2 c = __ldcg(p.units + u);
   const int n = c.y - c.x + 1;
   if (n <= 1 || r0 >= p.rows_all) return;
@@ -1186,43 +1316,6 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
     o.x += a.x; o.y += a.y; o.z += a.z; o.w += a.w;
   }
   put(x0, o);
-}
-
-// ------------------------------------------------------------------------------------
-// weights[b, h, j] += sum over the head's query rows of 2^(x_j - lse2): a thread a key, the
-// scores the split kernel left behind (L2 holds most of them) against the joined lse.
-// The step's own rows are set, not added to, and get their positions.
-__global__ void __launch_bounds__(256) attn_weights_kernel(const __grid_constant__ AttnParams p) {
-  __shared__ float z[512];
-  const int b = blockIdx.z, h = blockIdx.y;
-  pdl_wait();
-  pdl_launch_dependents();
-  const SeqSpan s = seq_span(clamp_length(p, b, false), p.q_len, p.window);
-  for (int r = threadIdx.x; r < p.rows_pad; r += blockDim.x) {
-    float v = INFINITY;                          // a padded or empty row adds nothing
-    if (r < p.rows_all) {
-      const int tok = r / p.group, head = h * p.group + r % p.group;
-      v = __ldcg(p.lse2 + (static_cast<long long>(b) * p.q_len + tok) * p.q_heads + head);
-      if (v == -INFINITY) v = INFINITY;
-    }
-    z[r] = v;
-  }
-  __syncthreads();
-  for (int j = s.lo + blockIdx.x * blockDim.x + threadIdx.x; j < s.n; j += gridDim.x * blockDim.x) {
-    const float* src = p.scores +
-                       ((static_cast<long long>(b) * p.kv_heads + h) * p.score_rows + j) * p.rows_pad;
-    float w = 0.f;
-    for (int r = 0; r < p.rows_pad; r += 4) {
-      const float4 x4 = __ldcg(reinterpret_cast<const float4*>(src + r));
-      const float x[4] = {x4.x, x4.y, x4.z, x4.w};
-#pragma unroll
-      for (int y = 0; y < 4; ++y) w += z[r + y] == INFINITY ? 0.f : ex2(x[y] - z[r + y]);
-    }
-    float* dst = p.weights + b * p.w_b + h * p.w_h + j;
-    const bool is_new = j >= s.n - p.q_len;
-    *dst = is_new ? w : *dst + w;
-    if (is_new && p.positions) p.positions[b * p.p_b + h * p.p_h + j] = __ldg(p.seen + b) - s.n + j;
-  }
 }
 
 // ------------------------------------------------------------------------------------
@@ -1395,9 +1488,12 @@ static int attn_run(AttnParams& p, int n_sm, int dev, bool pdl, void* stream) {
   const int blocks = ((p.rows_all < G::RB ? p.rows_all : G::RB) + 7) / 8;
   // the CTAs that share a unit: from nine on its partial results are worth a block an m-tile
   const int wide = static_cast<long long>(grid) * G::HG > 8LL * heads;
-  return wide ? attn_launch(attn_join_kernel<G, true>, dim3(heads, blocks, G::MT), kJoinThreads, 0, stream,
+  p.joins = static_cast<unsigned>(heads);
+  p.weight_chunks = p.scores ? static_cast<unsigned>((p.max_rows + kWeightKeys - 1) / kWeightKeys) : 0;
+  const unsigned x = p.joins + p.weight_chunks * static_cast<unsigned>(p.batch * p.kv_heads);
+  return wide ? attn_launch(attn_join_kernel<G, true>, dim3(x, blocks, G::MT), kJoinThreads, 0, stream,
                             true, p)
-              : attn_launch(attn_join_kernel<G, false>, dim3(heads, blocks), kJoinThreads, 0, stream, true, p);
+              : attn_launch(attn_join_kernel<G, false>, dim3(x, blocks), kJoinThreads, 0, stream, true, p);
 }
 
 // Sixteen rows a warp: their fragments of K and V are read and widened once.  Thirty-two (with
@@ -1535,11 +1631,5 @@ extern "C" int iq_attn_decode(const iq_attn_args* a, void* stream) {
       rc = bf16 ? attn_pick<IQ_ACT_BF16, 256>(p, n_sm, dev, pdl, stream)
                 : attn_pick<IQ_ACT_E4M3, 256>(p, n_sm, dev, pdl, stream);
   }
-  if (rc != IQ_OK || !weights) return rc;
-  // enough blocks for four waves of the chip, never more than the rows need
-  const int by_rows = static_cast<int>((rows + 255) / 256);
-  const int units = a->batch * a->kv_heads;
-  int x = (n_sm * 8 + units - 1) / units;
-  if (x > by_rows) x = by_rows;
-  return attn_launch(attn_weights_kernel, dim3(x, a->kv_heads, a->batch), 256, 0, stream, true, p);
+  return rc;
 }

@@ -24,11 +24,14 @@ namespace iqb {
 
 namespace cg = cooperative_groups;
 
-constexpr int kEvictThreads = 1024;
+// Threads of a selecting CTA: the many for long sequences, the few (eight CTAs an SM) where a
+// CTA of those holds all of a sequence's rows (65 x 16 heads of 256 rows: 39 us against 13).
+constexpr int kEvictMany = 1024, kEvictFew = 256;
 constexpr int kEvictChunk = 32768;               // weights a CTA of a cluster holds at most
 constexpr int kEvictCluster = 8;
 constexpr int kEvictRows = kEvictChunk * kEvictCluster;
 constexpr int kMoveThreads = 256;
+constexpr int kMovesInFlight = 2;
 // Moves a (sequence, head) can have at most for the selecting cluster to make them itself.
 constexpr int kEvictFusedMoves = 256;
 
@@ -73,6 +76,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 // Exclusive sum of `x` over the block's threads in thread order; *all gets the total.
+template <int T>
 __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* sums /* [32] */, uint32_t* all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto inclusive = [&](uint32_t v) {
@@ -86,7 +90,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* sums /* [32
   const uint32_t incl = inclusive(x);
   if (lane == 31) sums[warp] = incl;
   __syncthreads();
-  const uint32_t warps = inclusive(sums[lane]);  // (every warp for itself)
+  const uint32_t warps = inclusive(lane < T / 32 ? sums[lane] : 0);   // (every warp for itself)
   const uint32_t before = __shfl_sync(0xffffffffu, warps, warp ? warp - 1 : 0);
   *all = __shfl_sync(0xffffffffu, warps, 31);
   __syncthreads();                               // `sums` is free again
@@ -94,11 +98,12 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* sums /* [32
 }
 
 // Moves [i0, i0 + step, ..) of `total`, a cache row of K and of V each, by groups of `width`
-// threads (16 bytes a thread), four moves in flight a group: a move is a chain of its list
-// entry, two page lookups and the row itself.
+// threads (16 bytes a thread), two moves in flight a group: a move is a chain of its list
+// entry, two page lookups and the row itself, and more moves in flight cost more in resident
+// warps than they hide (24 x 8 heads, 1500 of 256 bytes each: two 33.9 us, four 44.8, one 42.7).
 __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int h, const int2* moves, int i0,
                                           int step, int total, int at, int width) {
-  constexpr int U = 4;
+  constexpr int U = kMovesInFlight;
 #pragma unroll 1
   for (int i = i0; i < total; i += U * step) {
     int to[U], from[U];
@@ -131,12 +136,14 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int h, co
   }
 }
 
-__global__ void __launch_bounds__(kEvictThreads) evict_kernel(const __grid_constant__ EvictParams p) {
+template <int T>
+__global__ void __launch_bounds__(T) evict_kernel(const __grid_constant__ EvictParams p) {
   extern __shared__ uint32_t keys[];             // [chunk]
   __shared__ uint32_t hist[3][2048];
   __shared__ uint32_t sums[32];
-  __shared__ uint32_t places[kEvictThreads];     // a warp's flags in a round of keys; then what lies before
-  __shared__ uint32_t equals[kEvictThreads];
+  constexpr int WARPS = T / 32;
+  __shared__ uint32_t places[T];     // a warp's flags in a round of keys; then what lies before
+  __shared__ uint32_t equals[T];
   __shared__ uint32_t found[3];                  // the digit, what is needed inside it, and all it has
   __shared__ uint32_t counts[2];                 // this CTA's keys at the edge; free places | moved rows << 16
   cg::cluster_group cluster = cg::this_cluster();
@@ -149,7 +156,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const __grid_const
   };
 
 #pragma unroll
-  for (int i = tid; i < 3 * 2048; i += kEvictThreads) hist[0][i] = 0;
+  for (int i = tid; i < 3 * 2048; i += T) hist[0][i] = 0;
   pdl_wait();
   pdl_launch_dependents();
   // This CTA's rows; their weights and positions are on their way before the length is known
@@ -164,7 +171,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const __grid_const
   int pv[AHEAD];
 #pragma unroll
   for (int x = 0; x < AHEAD; ++x) {
-    const int i = tid + x * kEvictThreads;
+    const int i = tid + x * T;
     if (i < end) {
       wv[x] = w[i0 + i];
       pv[x] = pos[i0 + i];
@@ -185,9 +192,9 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const __grid_const
   };
 #pragma unroll
   for (int x = 0; x < AHEAD; ++x)
-    if (tid + x * kEvictThreads < mine) take(tid + x * kEvictThreads, wv[x], pv[x]);
+    if (tid + x * T < mine) take(tid + x * T, wv[x], pv[x]);
 #pragma unroll 4
-  for (int i = tid + AHEAD * kEvictThreads; i < mine; i += kEvictThreads) take(i, w[i0 + i], pos[i0 + i]);
+  for (int i = tid + AHEAD * T; i < mine; i += T) take(i, w[i0 + i], pos[i0 + i]);
   if (n <= p.budget) {                           // (the whole cluster)
     if (rank == 0 && tid == 0) p.count[unit] = 0;
     return;
@@ -203,28 +210,37 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const __grid_const
     const int above = shift, width = pass < 2 ? 11 : 10;
     shift -= width;
 #pragma unroll 4
-    for (int i = tid; i < mine; i += kEvictThreads) {
+    for (int i = tid; i < mine; i += T) {
       const uint32_t key = keys[i];
       if (pass == 0 || key >> above == prefix) atomicAdd(&hist[pass][key >> shift & ((1u << width) - 1)], 1u);
     }
     sync();
-    // thread t: bins 2047 - 2 t and the one below, so that the sums run from the top
-    uint32_t c0 = 0, c1 = 0;
+    // thread t: BINS bins from 2047 - BINS t down, so that the sums run from the top
+    constexpr int BINS = 2048 / T;
+    uint32_t c[BINS] = {}, mine_of = 0;
 #pragma unroll
-    for (int c = 0; c < kEvictCluster; ++c) {
-      if (c >= cs) break;
-      const uint2 v = *reinterpret_cast<const uint2*>(
-          cluster.map_shared_rank(&hist[pass][0], c) + 2046 - 2 * tid);
-      c0 += v.y;
-      c1 += v.x;
+    for (int other = 0; other < kEvictCluster; ++other) {
+      if (other >= cs) break;
+      const uint2* v = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&hist[pass][0], other) +
+                                                      2048 - BINS * (tid + 1));
+#pragma unroll
+      for (int x = 0; x < BINS; x += 2) {
+        const uint2 two = v[(BINS - 2 - x) / 2];
+        c[x] += two.y;
+        c[x + 1] += two.x;
+      }
     }
-    uint32_t all;
-    const uint32_t before = block_scan(c0 + c1, sums, &all);
-    if (before < need && need <= before + c0 + c1) {
-      const bool second = need > before + c0;
-      found[0] = 2047 - 2 * tid - second;
-      found[1] = need - before - (second ? c0 : 0);
-      found[2] = second ? c1 : c0;
+#pragma unroll
+    for (int x = 0; x < BINS; ++x) mine_of += c[x];
+    uint32_t all, before = block_scan<T>(mine_of, sums, &all);
+#pragma unroll
+    for (int x = 0; x < BINS; ++x) {
+      if (before < need && need <= before + c[x]) {
+        found[0] = 2047 - BINS * tid - x;
+        found[1] = need - before;
+        found[2] = c[x];
+      }
+      before += c[x];
     }
     __syncthreads();
     prefix = prefix << width | found[0];
@@ -239,35 +255,35 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const __grid_const
 
   // ---- ranks, by rounds of a key a thread: a warp's flags are one ballot, and the counts of
   // (round, warp) are summed in the order of the keys
-  const int rounds = (p.chunk + kEvictThreads - 1) / kEvictThreads;   // <= 32
+  const int rounds = (p.chunk + T - 1) / T;   // <= 32
   const uint32_t below_me = (1u << lane) - 1;
   uint32_t all;
   if (ties) {
     for (int x = 0; x < rounds; ++x) {
-      const int i = x * kEvictThreads + tid;
+      const int i = x * T + tid;
       const uint32_t eq = __ballot_sync(0xffffffffu, i < mine && keys[i] == prefix);
-      if (lane == 0) equals[x * 32 + warp] = __popc(eq);
+      if (lane == 0) equals[x * WARPS + warp] = __popc(eq);
     }
     __syncthreads();
-    uint32_t before = block_scan(tid < rounds * 32 ? equals[tid] : 0, sums, &all);
+    uint32_t before = block_scan<T>(tid < rounds * WARPS ? equals[tid] : 0, sums, &all);
     if (cs > 1) {
       if (tid == 0) counts[0] = all;
       cluster.sync();
       for (int c = 0; c < rank; ++c) before += cluster.map_shared_rank(counts, c)[0];
     }
-    if (tid < rounds * 32) equals[tid] = before;
+    if (tid < rounds * WARPS) equals[tid] = before;
     __syncthreads();
   }
   uint32_t free_place = 0, moved = 0;            // this round's ballots
   auto flags = [&](int x) {
-    const int i = x * kEvictThreads + tid;
+    const int i = x * T + tid;
     const bool live = i < mine;
     const uint32_t key = live ? keys[i] : 0, top = key >> shift;
     bool kept = top > prefix || top == prefix;
     if (ties) {
       const bool eq = live && key == prefix;
       const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
-      if (eq) kept = equals[x * 32 + warp] + __popc(eqs & below_me) < need;
+      if (eq) kept = equals[x * WARPS + warp] + __popc(eqs & below_me) < need;
     }
     const bool low = i0 + i < p.budget;
     free_place = __ballot_sync(0xffffffffu, live && low && !kept);
@@ -275,10 +291,10 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const __grid_const
   };
   for (int x = 0; x < rounds; ++x) {
     flags(x);
-    if (lane == 0) places[x * 32 + warp] = __popc(free_place) | __popc(moved) << 16;
+    if (lane == 0) places[x * WARPS + warp] = __popc(free_place) | __popc(moved) << 16;
   }
   __syncthreads();
-  uint32_t before = block_scan(tid < rounds * 32 ? places[tid] : 0, sums, &all);
+  uint32_t before = block_scan<T>(tid < rounds * WARPS ? places[tid] : 0, sums, &all);
   int total = static_cast<int>(all >> 16), free_at = 0, move_at = 0;
   if (cs > 1) {
     if (tid == 0) counts[1] = all;
@@ -295,25 +311,25 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const __grid_const
       total += static_cast<int>(other >> 16);
     }
   }
-  if (tid < rounds * 32) places[tid] = before;
+  if (tid < rounds * WARPS) places[tid] = before;
   __syncthreads();
   int2* moves = p.moves + static_cast<long long>(unit) * p.move_rows;
   for (int x = 0; x < rounds; ++x) {
     flags(x);
-    const uint32_t base = places[x * 32 + warp];
-    const int at = i0 + x * kEvictThreads + tid;
+    const uint32_t base = places[x * WARPS + warp];
+    const int at = i0 + x * T + tid;
     if (free_place >> lane & 1) moves[free_at + (base & 0xffff) + __popc(free_place & below_me)].x = at;
     if (moved >> lane & 1) moves[move_at + (base >> 16) + __popc(moved & below_me)].y = at;
   }
   if (rank == 0 && tid == 0) p.count[unit] = total;
   sync();                                        // the list is complete; no CTA's memory is read any more
-  for (int i = rank * kEvictThreads + tid; i < total; i += cs * kEvictThreads) {
+  for (int i = rank * T + tid; i < total; i += cs * T) {
     const int2 mv = __ldcg(moves + i);
     w_out[mv.x] = w[mv.y];
     pos_out[mv.x] = pos[mv.y];
   }
   if (p.fused) {
-    const int width = p.row_bytes <= 128 ? 8 : 32, per = kEvictThreads / width;
+    const int width = p.row_bytes <= 128 ? 8 : 32, per = T / width;
     move_rows(p, b, h, moves, rank * per + tid / width, cs * per, total, tid % width, width);
   }
 }
@@ -378,7 +394,7 @@ static int kv_sms() {
   if (per_device[dev] == 0) {
     int n = 0;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    if (cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    if (cudaFuncSetAttribute(evict_kernel<kEvictMany>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              kEvictChunk * 4) != cudaSuccess)
       return 0;
     per_device[dev] = n;
@@ -496,15 +512,18 @@ extern "C" int iq_kv_evict(const iq_evict_args* a, void* stream) {
   int cluster = 1;
   while (cluster < kEvictCluster &&
          (rows > static_cast<long long>(kEvictChunk) * cluster ||
-          (rows > 8LL * kEvictThreads * cluster && units * cluster <= n_sm)))
+          (rows > 8LL * kEvictMany * cluster && units * cluster <= n_sm)))
     cluster *= 2;
   p.chunk = static_cast<int>((rows + cluster - 1) / cluster);
-  const int rc = kv_launch(evict_kernel, p, dim3(static_cast<unsigned>(units * cluster)), kEvictThreads,
-                           p.chunk * 4, cluster, stream, a->pdl != 0);
+  const dim3 grid(static_cast<unsigned>(units * cluster));
+  const int rc = rows <= 8 * kEvictFew
+                     ? kv_launch(evict_kernel<kEvictFew>, p, grid, kEvictFew, p.chunk * 4, 1, stream, a->pdl != 0)
+                     : kv_launch(evict_kernel<kEvictMany>, p, grid, kEvictMany, p.chunk * 4, cluster, stream,
+                                 a->pdl != 0);
   if (rc != IQ_OK || p.fused) return rc;
-  // four rows for every group of lanes, twice the chip's threads at most
+  // two rows for every group of lanes, twice the chip's threads at most
   const int per = kMoveThreads / (p.row_bytes <= 128 ? 8 : p.row_bytes <= 256 ? 16 : 32);
-  long long x = (most + 4 * per - 1) / (4 * per);
+  long long x = (most + kMovesInFlight * per - 1) / (kMovesInFlight * per);
   const long long cap = (n_sm * 16 + units - 1) / units;
   if (x > cap) x = cap;
   return kv_launch(evict_move_kernel, p, dim3(static_cast<unsigned>(x), static_cast<unsigned>(units)),

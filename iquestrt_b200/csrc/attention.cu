@@ -328,7 +328,8 @@ __device__ __noinline__ void add_not_finite(const AttnParams& p, int b, int n, i
     }
     if (sum == 0.f) continue;
     if (whole) {
-      p.out[b * p.o_b + tok * p.o_r + head * p.o_h + d] = __float2bfloat16_rn(sum);
+      __nv_bfloat16* o = p.out + b * p.o_b + tok * p.o_r + head * p.o_h + d;
+      *o = __float2bfloat16_rn(__bfloat162float(*o) + sum);
     } else {
       // the place of (rr, d) in the fragments
       int x, y, g;
@@ -368,8 +369,10 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
   mbar_fence_init();
   if (tid == 0) {
     *not_finite = 0;
-    prefetch_tensormap(&p.k_map);
-    prefetch_tensormap(&p.v_map);
+    if (!p.gather) {
+      prefetch_tensormap(&p.k_map);
+      prefetch_tensormap(&p.v_map);
+    }
   }
   pdl_wait();
   pdl_launch_dependents();
@@ -1478,8 +1481,9 @@ static int attn_run(AttnParams& p, int n_sm, int dev, bool pdl, void* stream) {
   p.gather = 2 * G::BOXES * (G::KPW / box) * (G::HG / p.box_heads) * G::KG > 16;
   static std::atomic<uint64_t> done{0};          // (a launch with fewer registers would wait for good)
   if (!attn_ready(attn_kernel<G>, done, dev, G::SMEM, G::MOVE_REGS ? G::REGS : 0)) return IQ_ERR_CUDA;
-  int rc = attn_map(&p.k_map, p.k, p, p.k_row, p.k_head, G::ELT, G::PITCH);
-  if (rc == IQ_OK) rc = attn_map(&p.v_map, p.v, p, p.v_row, p.v_head, G::ELT, G::PITCH);
+  int rc = IQ_OK;
+  if (!p.gather) rc = attn_map(&p.k_map, p.k, p, p.k_row, p.k_head, G::ELT, G::PITCH);
+  if (!p.gather && rc == IQ_OK) rc = attn_map(&p.v_map, p.v, p, p.v_row, p.v_head, G::ELT, G::PITCH);
   if (rc != IQ_OK) return rc;
   const int grid = static_cast<int>(tiles < n_sm ? tiles : n_sm);
   rc = attn_launch(attn_kernel<G>, dim3(grid), G::THREADS, G::SMEM, stream, pdl, p);

@@ -490,7 +490,7 @@ class AttnWork:
 
 def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, scale=None,
                 window: int = 0, out=None, lse=None, weights=None, positions=None, seen=None,
-                work: AttnWork | None = None, scratch: Scratch | None = None, pdl: bool = False):
+                work: AttnWork | None = None, scratch: Scratch | None = None, pdl: bool = True):
     """Attention of the last `q_len` tokens of each sequence over its paged KV cache
     (`iq_attn_decode`): `q [batch, q_len, q_heads, D]` bf16 -> `out`, same shape.
 
@@ -505,7 +505,9 @@ def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, sca
     the query heads of its key/value head and the new tokens; the new tokens' own entries are
     set, and those of `positions` (int32, same shape) to the tokens' positions, `seen [batch]`
     (int32) being the tokens seen so far with the new ones.  Without `work` one is allocated
-    for the call.  A length or page out of range shows in `scratch`'s status word.
+    for the call.  A length or page out of range shows in `scratch`'s status word.  `pdl` lets
+    the launch's set-up overlap the kernel before it; nothing is read or written before that
+    kernel is done.
 
     Addresses of q, out and the caches, and their strides, are multiples of 16 bytes."""
     if not isinstance(q, torch.Tensor) or q.dim() != 4:
@@ -576,7 +578,7 @@ class EvictWork:
 def kv_evict(k_cache, v_cache, page_table, lengths, weights, positions, seen, *, page_size: int,
              budget: int, lengths_out, keep_first: int = 0, keep_last: int = 0, weights_out=None,
              positions_out=None, work: EvictWork | None = None, scratch: Scratch | None = None,
-             pdl: bool = False):
+             pdl: bool = True):
     """Cuts every sequence of more than `budget` rows down to `budget` (`iq_kv_evict`): each
     key/value head keeps its rows of position < `keep_first` or >= `seen - keep_last`, then
     those of the largest accumulated weight (ties to the lower row).
@@ -628,7 +630,7 @@ def kv_evict(k_cache, v_cache, page_table, lengths, weights, positions, seen, *,
 
 def kv_advance(page_table, lengths, seen, slot, pos, *, page_size: int, capacity: int,
                q_len: int = 1, max_positions: int = 0, lengths_out=None, seen_out=None,
-               scratch: Scratch | None = None, pdl: bool = False):
+               scratch: Scratch | None = None, pdl: bool = True):
     """The cache rows and positions of the next `q_len` tokens of every sequence
     (`iq_kv_advance`), on the device, so that a captured step finds its own rows: `slot` and
     `pos [batch * q_len]` (int64) are what `qkv_heads` and the rotary tables take.  `lengths`

@@ -95,6 +95,8 @@ SHAPES = [
     ([333, 64, 0, 1], 2, 4, 2, 64, 5, 77),
     ([333, 47], 1, 8, 2, 128, 1, 100),
     ([0, 0], 2, 4, 2, 64, 8, 0),
+    ([2000, 700, 90], 2, 24, 6, 128, 64, 0),
+    ([3000, 10], 8, 40, 1, 128, 32, 0),      # 320 query rows a head: five blocks
 ]
 
 
@@ -139,6 +141,16 @@ def test_a_row_is_not_touched_by_what_it_does_not_see(scratch, kv, q_len, window
     assert torch.equal(got[0, sound], clean[0, sound])
     if window:
         assert torch.isnan(got[0, 0].float()).all()
+    if kv == BF16 and not window:
+        # infinities in single channels of the newest value; a NaN that all see stays one
+        k[rows[399]], v[rows[399]] = 0.5, 0.25
+        v[rows[399], 0, 7], v[rows[399], 1, 9] = float("inf"), float("-inf")
+        v[rows[10], 0, 7] = float("nan")
+        got = ops.attn_decode(q, k, v, table, n, **call).float()
+        assert torch.isnan(got[0, :, :4, 7]).all()
+        assert (got[0, -1, 4:, 9] == float("-inf")).all()
+        got[0, :, :4, 7] = got[0, -1, 4:, 9] = 0
+        assert torch.isfinite(got).all()
 
 
 def test_scores_of_any_size(scratch):
@@ -261,6 +273,8 @@ EVICT = [
     ([5000, 4097, 4096], 2, 64, 64, 4096, 16, 1000),
     ([3000, 700], 2, 256, 1, 500, 3, 7),
     ([9000, 20000], 2, 128, 16, 6000, 16, 64),
+    ([100_000], 1, 32, 64, 70_000, 16, 64),
+    ([40_000, 33_000, 2], 3, 16, 128, 30_000, 0, 0),
 ]
 
 

@@ -34,7 +34,8 @@ def _attn_args():
     ("lengths", None, 1), ("out", None, 1), ("work", None, 1), ("page_size", 0, 1),
     ("max_pages", 0, 1), ("capacity", 0, 1), ("window", -1, 1), ("kv_kind", 2, 1),
     ("work_bytes", 100, 1), ("k_cache", 4096 + 8, 1), ("v_cache", 4096 + 8, 1), ("k_row", 120, 1),
-    ("v_row", 120, 1), ("v_head", 8, 1), ("q", 4098, 1), ("q_h", 127, 1), ("work", 4104, 1),
+    ("v_row", 120, 1), ("v_head", 8, 1), ("q", 4104, 1), ("q_h", 127, 1), ("q_r", 1028, 1), ("out", 4104, 1), ("o_h", 132, 1),
+    ("k_row", -128, 1), ("v_head", 1 << 41, 1), ("work", 4104, 1),
     ("positions", 4096, 1), ("seen", 4096, 1),
     ("batch", 0, 6), ("batch", 1025, 6), ("q_len", 0, 6), ("q_len", 9, 6), ("q_heads", 0, 6),
     ("head_dim", 8, 6), ("head_dim", 100, 6), ("head_dim", 272, 6), ("q_heads", 513, 6),

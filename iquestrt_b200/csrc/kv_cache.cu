@@ -100,7 +100,8 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* sums /* [32
 // Moves [i0, i0 + step, ..) of `total`, a cache row of K and of V each, by groups of `width`
 // threads (16 bytes a thread), two moves in flight a group: a move is a chain of its list
 // entry, two page lookups and the row itself, and more moves in flight cost more in resident
-// warps than they hide (24 x 8 heads, 1500 of 256 bytes each: two 33.9 us, four 44.8, one 42.7).
+// warps than they hide (24 x 8 heads, some 1500 of
+// 256 bytes each: two 33 to 39 us with where the pages lie, four 45, one 43).
 __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int h, const int2* moves, int i0,
                                           int step, int total, int at, int width) {
   constexpr int U = kMovesInFlight;

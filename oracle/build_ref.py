@@ -44,6 +44,11 @@ def module_path(name: str) -> str:
     return os.path.join(OUT, name + ".so")
 
 
+def present(reference: str = DEFAULT_REFERENCE) -> bool:
+    """True when the reference's kernel modules can be read there."""
+    return os.path.isdir(os.path.join(reference, "iquestrt", "kernels"))
+
+
 def available() -> bool:
     """True when every reference extension has been built."""
     return all(os.path.exists(module_path(n)) for n in UNITS)
@@ -76,7 +81,7 @@ def _stale(name: str, reference: str) -> bool:
 
 def build(reference: str = DEFAULT_REFERENCE, force: bool = False, verbose: bool = False):
     """Build whatever is missing or older than the reference's files; returns the paths."""
-    if not os.path.isdir(reference):
+    if not present(reference):
         raise RuntimeError(f"reference checkout not found at {reference}")
     os.makedirs(OUT, exist_ok=True)
     todo = [n for n in UNITS if force or _stale(n, reference)]

@@ -54,13 +54,14 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB
     os.makedirs(OBJ, exist_ok=True)
     nvcc = _nvcc()
+    new = f".{os.getpid()}.new"                  # another process may be building too
     objects, running = [], []
     for source in SOURCES:
         obj = os.path.join(OBJ, source.replace(".cu", ".o"))
         objects.append(obj)
         if not force and not _newer(obj, _deps(source)):
             continue
-        cmd = [nvcc, *NVCC_FLAGS, "-c", "-o", obj + ".new", os.path.join(CSRC, source)]
+        cmd = [nvcc, *NVCC_FLAGS, "-c", "-o", obj + new, os.path.join(CSRC, source)]
         if verbose:
             cmd[1:1] = ["-Xptxas", "-v"]
         running.append((obj, subprocess.Popen(cmd, stdout=subprocess.PIPE,
@@ -71,13 +72,13 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if proc.returncode != 0:
             failed.append(text)
             continue
-        os.replace(obj + ".new", obj)
+        os.replace(obj + new, obj)
         if verbose:
             print(text)
     if failed:
         raise RuntimeError("nvcc failed:\n" + "\n".join(failed))
     # link beside the target and rename: a reader never sees a half-written library
-    staged = LIB + ".new"
+    staged = LIB + new
     proc = subprocess.run([nvcc, *NVCC_FLAGS, "-shared", "-o", staged, *objects],
                           capture_output=True, text=True)
     if proc.returncode != 0:

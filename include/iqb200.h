@@ -302,9 +302,11 @@ int iq_moe_down(const iq_moe_down_args* a, void* stream);
  * 0.  out = softmax(scale q.k) v per query head (q_heads / kv_heads of them share a key/value
  * head), lse = log of the softmax's sum; a row that sees nothing (a sequence of fewer than
  * q_len rows, an empty one) gets zeros and -infinity.  Rows outside a query row's view never
- * reach it, infinities and NaNs there included; rows past lengths[b] are not read.  Softmax
+ * reach it, infinities and NaNs there included, nor do rows past lengths[b].  Softmax
  * statistics, scores and sums are fp32; the weights enter the product with v as half
- * precision (e4m3 caches) or bf16 (bf16 caches).
+ * precision (e4m3 caches) or bf16 (bf16 caches).  With e4m3 caches q enters its product as
+ * half precision too, each row scaled by a power of two: exact but for elements some 2^30
+ * below the row's largest.
  *
  * With `weights`, weights[b][h][j] gains the sum of the softmax weights that the query heads
  * and rows of key/value head h gave row j; for the step's own rows it is set to it, and
@@ -312,8 +314,8 @@ int iq_moe_down(const iq_moe_down_args* a, void* stream);
  * has seen in all, which eviction leaves larger than its length.
  *
  * head_dim is a multiple of 16 up to 256, q_len 1..8, batch up to 1024, (q_heads / kv_heads)
- * * q_len up to 512.  Strides are in elements; those of the caches times the element size,
- * and the caches' addresses, are multiples of 16 bytes.  `work` (iq_attn_work_bytes, 16-byte
+ * * q_len up to 512.  Strides are in elements; those of the caches, q and out times the
+ * element size, and their addresses, are multiples of 16 bytes.  `work` (iq_attn_work_bytes, 16-byte
  * aligned) needs no initialisation; calls that share it must be ordered.  A length outside
  * the page table is clamped and a page outside the cache read as zeros, with IQ_ERR_ROUTE in
  * the status word. */
@@ -359,8 +361,8 @@ int iq_attn_decode(const iq_attn_args* a, void* stream);
  * `budget` keep their place; the others move into the freed places below it, the i-th such
  * row (ascending) into the i-th place.  K and V move in place; weights and positions of the
  * rows that stay go to weights_out / positions_out (which may be weights / positions
- * themselves), entries from `budget` (or n) on are left as they were; lengths_out[b] = min(n,
- * budget) (not `lengths`: every head reads that).  Sequences must not share pages.
+ * themselves, with their strides, but share no memory with them otherwise), entries from `budget` (or n) on are left as they were; lengths_out[b] = min(n,
+ * budget) (not in the memory of `lengths` or `seen`: every head reads those).  Sequences must not share pages.
  *
  * Strides in elements, the caches' 16-byte aligned as in iq_attn_decode; rows = page_size *
  * max_pages up to 262144; `work` (iq_evict_work_bytes) needs no initialisation. */
@@ -396,7 +398,8 @@ int iq_kv_evict(const iq_evict_args* a, void* stream);
 
 /* The cache rows and positions of the next q_len tokens of every sequence: slot[b * q_len + r]
  * = the cache row of row lengths[b] + r (what iq_qkv_heads takes), pos[...] = seen[b] + r,
- * lengths_out = lengths + q_len, seen_out = seen + q_len (both may be the inputs themselves).
+ * lengths_out = lengths + q_len, seen_out = seen + q_len (both may be the inputs themselves,
+ * but not overlap them, or one another, otherwise).
  * A sequence whose pages do not reach so far, or whose positions would pass max_positions
  * (0: no limit), keeps its length and gets slots of -1 and positions of 0, with IQ_ERR_ROUTE
  * in the status word. */

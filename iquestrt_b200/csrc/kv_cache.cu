@@ -10,6 +10,9 @@
 // with the kept rows above it: sources and destinations are disjoint, so it runs in place, in
 // any order and on all SMs, and moves the fewest rows there are to move.
 // What bounds it: latency (barriers, passes) for a step's few rows, HBM for a long prompt's.
+// Measured (one B200, pages of 64, 8 heads, 128 channels of e4m3): one row of 4097 out: 10.5
+// us; 32768 rows to 8192: 22.7 us, 0.19 of the copy rate, half of it the selection; 24 ragged
+// sequences of bf16 to 2048 rows: 33 to 39 us with where the pages lie, 3.3 to 3.9 TB/s.
 #include <math.h>
 #include <stdio.h>
 
@@ -356,7 +359,8 @@ struct AdvanceParams {
   int* status;
 };
 
-// A thread a sequence: it reads the sequence's length and count before it writes them.
+// A thread a sequence: it reads the sequence's length and count before it writes them.  All
+// latency, 1.5 us; 2.4 us for 256 sequences of four tokens.
 __global__ void __launch_bounds__(128) advance_kernel(const __grid_constant__ AdvanceParams p) {
   pdl_wait();
   pdl_launch_dependents();
@@ -440,6 +444,12 @@ static int kv_launch(void (*kernel)(const P), const P& p, dim3 grid, int threads
   return IQ_OK;
 }
 
+// Whether two arrays of n ints share memory.
+static bool overlap(const int* a, const int* b, long long n) {
+  const uint64_t x = reinterpret_cast<uint64_t>(a), y = reinterpret_cast<uint64_t>(b);
+  return (x < y ? y - x : x - y) < static_cast<uint64_t>(n) * 4;
+}
+
 static size_t evict_count_bytes(long long units) { return static_cast<size_t>((units * 4 + 255) / 256 * 256); }
 
 static bool evict_shape_ok(int batch, int kv_heads, long long rows) {
@@ -468,9 +478,13 @@ extern "C" int iq_kv_evict(const iq_evict_args* a, void* stream) {
   if (a->budget < 1 || a->keep_first < 0 || a->keep_last < 0 ||
       static_cast<long long>(a->keep_first) + a->keep_last > a->budget)
     return IQ_ERR_ARG;
-  if (a->lengths_out == a->lengths) return IQ_ERR_ARG;
   const long long rows = static_cast<long long>(a->page_size) * a->max_pages;
   if (!evict_shape_ok(a->batch, a->kv_heads, rows)) return IQ_ERR_UNSUPPORTED;
+  // every head reads both; in place means element on element
+  if (overlap(a->lengths_out, a->lengths, a->batch) || overlap(a->lengths_out, a->seen, a->batch) ||
+      (a->weights_out == a->weights && (a->wo_b != a->w_b || a->wo_h != a->w_h)) ||
+      (a->positions_out == a->positions && (a->po_b != a->p_b || a->po_h != a->p_h)))
+    return IQ_ERR_ARG;
   const int elt = a->kv_kind == IQ_ACT_BF16 ? 2 : 1;
   if (a->head_dim < 1 || a->head_dim > 1024 || a->head_dim * elt % 16) return IQ_ERR_UNSUPPORTED;
   if (a->work_bytes < iq_evict_work_bytes(a->batch, a->kv_heads, static_cast<int>(rows)))
@@ -540,6 +554,11 @@ extern "C" int iq_kv_advance(const iq_advance_args* a, void* stream) {
     return IQ_ERR_ARG;
   const long long rows = static_cast<long long>(a->page_size) * a->max_pages;
   if (rows > 0x3fffffffLL || a->batch > (1 << 24)) return IQ_ERR_UNSUPPORTED;
+  // in place means element on element: another thread's element is not to be written
+  for (const int* out : {a->lengths_out, a->seen_out})
+    for (const int* in : {a->lengths, a->seen})
+      if (out != in && overlap(out, in, a->batch)) return IQ_ERR_ARG;
+  if (overlap(a->lengths_out, a->seen_out, a->batch)) return IQ_ERR_ARG;
   AdvanceParams p{};
   p.pages = PageTable{a->page_table, a->table_stride, a->page_size, page_shift(a->page_size), a->capacity};
   p.max_rows = static_cast<int>(rows);

@@ -86,10 +86,12 @@ class PagedKvCache:
     def advance(self, *, max_positions: int = 0, pdl: bool = False) -> None:
         """Rows and positions of the step's tokens into `slot` / `pos`; `lengths` and `seen`
         count them from here on.  A sequence without room for them (or that would reach
-        `max_positions`) stays as it was, and the scratch's status word says so."""
+        `max_positions`) keeps its rows and counts, and the scratch's status word says so; what
+        the step then computes for it means nothing, the accumulated weights and positions of
+        its newest rows included."""
         ops.kv_advance(self.page_table, self.held, self.seen, self.slot, self.pos,
-                       page_size=self.page_size, capacity=self.capacity, q_len=self.q_len, max_positions=max_positions,
-                       lengths_out=self.lengths, scratch=self.scratch, pdl=pdl)
+                       page_size=self.page_size, capacity=self.capacity, q_len=self.q_len,
+                       max_positions=max_positions, lengths_out=self.lengths, scratch=self.scratch, pdl=pdl)
 
     def evict(self, layer: int, *, pdl: bool = False) -> None:
         """Cuts `layer`'s sequences back to the budget, after the step's attention; `held` gets

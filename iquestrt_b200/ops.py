@@ -587,8 +587,8 @@ def kv_evict(k_cache, v_cache, page_table, lengths, weights, positions, seen, *,
     keeps them.  Rows that stay below `budget` stay where they are; the others move, in place
     and in ascending order, into the places freed there, with their weights and positions
     (`weights_out` / `positions_out`, by default the inputs themselves).  `lengths_out [batch]`
-    (int32, not `lengths`: layers of a model share the lengths of before) gets the new
-    lengths.  Sequences must not share pages."""
+    (int32, not in the memory of `lengths` or `seen`: layers of a model share the lengths of
+    before) gets the new lengths.  Sequences must not share pages."""
     if not isinstance(weights, torch.Tensor) or weights.dim() != 3:
         raise ValueError("weights must be a tensor [batch, kv_heads, rows]")
     shape, index = weights.shape, weights.get_device()

@@ -113,6 +113,38 @@ def test_advance_refuses(field, value):
     assert lib.iq_kv_advance(C.byref(a), None) == L.IQ_ERR_ARG
 
 
+def test_outputs_that_overlap_what_others_read_are_refused():
+    """Lengths and counts in place mean element on element; a shifted view is an error, for the
+    eviction (every head reads them) any overlap is."""
+    L, lib = _lib()
+    a = L.AdvanceArgs()
+    for i, f in enumerate(("page_table", "lengths", "seen", "lengths_out", "seen_out", "slot", "pos")):
+        setattr(a, f, 4096 * (i + 1))
+    a.page_size, a.max_pages, a.capacity, a.batch, a.q_len = 16, 4, 64, 8, 1
+    for field, value in (("lengths_out", a.lengths + 4), ("lengths_out", a.seen - 28),
+                         ("seen_out", a.lengths - 4), ("seen_out", a.seen + 28),
+                         ("seen_out", a.lengths_out + 8), ("seen_out", a.lengths_out)):
+        was = getattr(a, field)
+        setattr(a, field, value)
+        assert lib.iq_kv_advance(C.byref(a), None) == L.IQ_ERR_ARG, (field, value)
+        setattr(a, field, was)
+
+    _, _, e = _evict_args()
+    e.batch = 8
+    for i, f in enumerate(("lengths", "seen", "lengths_out", "weights", "weights_out", "positions",
+                           "positions_out")):
+        setattr(e, f, 65536 * (i + 1))
+    for change in (dict(lengths_out=e.lengths + 4), dict(lengths_out=e.seen - 28),
+                   dict(lengths_out=e.seen), dict(weights_out=e.weights, wo_b=640),
+                   dict(positions_out=e.positions, po_h=640)):
+        was = {f: getattr(e, f) for f in change}
+        for f, value in change.items():
+            setattr(e, f, value)
+        assert lib.iq_kv_evict(C.byref(e), None) == L.IQ_ERR_ARG, change
+        for f, value in was.items():
+            setattr(e, f, value)
+
+
 def _tensors():
     bf = torch.bfloat16
     return dict(q=torch.zeros(2, 1, 8, 128, dtype=bf), k_cache=torch.zeros(64, 2, 128, dtype=bf),

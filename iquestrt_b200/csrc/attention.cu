@@ -1127,8 +1127,8 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
 // thread the four values of one lane of an m-tile; WIDE (many partial results a unit): a
 // block joins one m-tile, its eight warps every eighth partial result.  It is all latency
 // (the unit's place, then its partial results), so a thread has all its loads in flight at
-// once, those of the maxima and sums among them.  Measured: 2 us behind the split kernel for
-// 8 rows over 32k keys; a join by the unit's last CTA inside the split kernel saved the
+// once, those of the maxima and sums among them.  Measured: 5 to 6 us alone with
+// cold caches, most of it hidden behind the split kernel's end; a join by the unit's last CTA inside the split kernel saved the
 // launch and lost more (9.0 -> 11.6 us a call at a window of 4096 keys, 147 -> 160 for the
 // ragged batch), being serial in one CTA.
 constexpr int kJoinThreads = 256;

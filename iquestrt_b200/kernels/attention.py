@@ -27,17 +27,28 @@ class PagedKvCache:
                  keep_first: int = 4, keep_last: int = 0, scratch=None):
         if not 1 <= q_len <= 8:
             raise ValueError(f"q_len must be 1..8, got {q_len}")
+        if min(layers, batch, kv_heads, head_dim, rows, page_size) < 1:
+            raise ValueError(f"sizes must be at least 1, got {layers} layers, batch {batch}, "
+                             f"{kv_heads} heads of {head_dim}, {rows} rows, pages of {page_size}")
         if dtype not in (torch.bfloat16, torch.float8_e4m3fn):
             raise ValueError(f"the KV cache must be bf16 or e4m3, got {dtype}")
         if budget is not None and not 1 <= budget <= rows - q_len:
             raise ValueError(f"a budget of {budget} rows and {q_len} new ones need more than "
                              f"{rows} rows")
+        if budget is not None and (min(keep_first, keep_last) < 0
+                                   or keep_first + keep_last > budget):
+            raise ValueError(f"a budget of {budget} rows does not hold the protected ones, "
+                             f"{keep_first} + {keep_last}")
         pages = -(-rows // page_size)
         if page_table is None:
             page_table = torch.arange(batch * pages, dtype=torch.int32).view(batch, pages)
             capacity = batch * pages * page_size
         elif capacity is None:
             raise ValueError("a page table needs the caches' capacity")
+        elif page_table.dim() != 2 or page_table.shape[0] != batch \
+                or page_table.shape[1] * page_size < rows:
+            raise ValueError(f"page_table {tuple(page_table.shape)} does not give {batch} sequences "
+                             f"{rows} rows each in pages of {page_size}")
         self.batch, self.q_len, self.kv_heads, self.head_dim = batch, q_len, kv_heads, head_dim
         self.page_size, self.capacity = page_size, capacity
         self.budget, self.keep_first, self.keep_last = budget, keep_first, keep_last

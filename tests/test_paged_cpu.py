@@ -255,6 +255,21 @@ def test_oracle_eviction_by_hand():
     assert out[4].tolist() == [3]
 
 
+@pytest.mark.parametrize("change,message", [
+    (dict(page_size=0), "at least 1"), (dict(batch=0), "at least 1"), (dict(layers=0), "at least 1"),
+    (dict(budget=3), "protected"), (dict(budget=20, keep_last=17), "protected"),
+    (dict(budget=20, keep_first=-1), "protected"),
+    (dict(page_table=torch.zeros(2, 3, dtype=torch.int32)), "capacity"),
+    (dict(page_table=torch.zeros(1, 4, dtype=torch.int32), capacity=64), "page_table"),
+    (dict(page_table=torch.zeros(2, 3, dtype=torch.int32), capacity=64), "page_table"),
+])
+def test_cache_holder_refuses(change, message):
+    from iquestrt_b200.kernels import PagedKvCache
+    args = dict(layers=1, batch=2, kv_heads=1, head_dim=128, rows=64, page_size=16, device="cpu")
+    with pytest.raises(ValueError, match=message):
+        PagedKvCache(**{**args, **change})
+
+
 def test_holders_refuse():
     from iquestrt_b200.kernels import PagedAttention, PagedKvCache
     from iquestrt_b200.workspace import Workspace

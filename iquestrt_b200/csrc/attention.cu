@@ -80,7 +80,8 @@ struct AttnParams {
   int* positions;
   long long p_b, p_h;
   const int* seen;
-  unsigned joins, weight_chunks;                 // blocks that join; blocks a (sequence, head)'s weights take
+  unsigned joins;                                // blocks along x that join
+  unsigned weight_chunks, weight_blocks;         // blocks a (sequence, head)'s weights take; all of them
   int* status;
   int batch, q_len, q_heads, kv_heads, group, dim, window;
   int rows_all;                                  // group * q_len
@@ -1138,8 +1139,8 @@ constexpr int kJoinParts = 160;                  // partial results of a unit, a
 // scores the split kernel left behind (L2 holds most of them).  Each block works out the rows'
 // lse2 from the partial results for itself, so these blocks need not wait for those that join.
 // The step's own rows are set, not added to, and get their positions.  64 / 8 heads over 32768
-// keys of e4m3: 28.0 us with the weights, 8 MB of scores written and read once more.
-constexpr int kWeightKeys = 1024;                // keys a block
+// keys of e4m3: 26.6 us with the weights, 8 MB of scores written and read once more.
+constexpr int kWeightKeys = 1024;                // keys a block (512: 27.5 us; 81.9 over 128k, 1024 74.6)
 
 template <class G>
 __device__ __forceinline__ void add_weights(const AttnParams& p, int chunk, int bh, float* z /* [512] */) {
@@ -1231,9 +1232,9 @@ __global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const __grid_co
   pdl_wait();
   pdl_launch_dependents();
   if (blockIdx.x >= p.joins) {
-    if (blockIdx.y == 0 && blockIdx.z == 0)
-      add_weights<G>(p, (blockIdx.x - p.joins) % p.weight_chunks, (blockIdx.x - p.joins) / p.weight_chunks,
-                     reinterpret_cast<float*>(red));
+    const unsigned i = (blockIdx.z * gridDim.y + blockIdx.y) * (gridDim.x - p.joins) + blockIdx.x - p.joins;
+    if (i < p.weight_blocks)
+      add_weights<G>(p, i % p.weight_chunks, i / p.weight_chunks, reinterpret_cast<float*>(red));
     return;
   }
   const int u = blockIdx.x / G::HG, hg = blockIdx.x % G::HG;
@@ -1510,7 +1511,11 @@ static int attn_run(AttnParams& p, int n_sm, int dev, bool pdl, void* stream) {
   const int wide = static_cast<long long>(grid) * G::HG > 8LL * heads;
   p.joins = static_cast<unsigned>(heads);
   p.weight_chunks = p.scores ? static_cast<unsigned>((p.max_rows + kWeightKeys - 1) / kWeightKeys) : 0;
-  const unsigned x = p.joins + p.weight_chunks * static_cast<unsigned>(p.batch * p.kv_heads);
+  p.weight_blocks = p.weight_chunks * static_cast<unsigned>(p.batch * p.kv_heads);
+  // the weights' blocks fill the grid's other axes too: empty blocks cost (64 / 8 heads over
+  // 32k keys: 28.1 us with them, 26.6 without; over 128k 80.8 and 74.6)
+  const unsigned layers = static_cast<unsigned>(blocks * (wide ? G::MT : 1));
+  const unsigned x = p.joins + (p.weight_blocks + layers - 1) / layers;
   return wide ? attn_launch(attn_join_kernel<G, true>, dim3(x, blocks, G::MT), kJoinThreads, 0, stream,
                             true, p)
               : attn_launch(attn_join_kernel<G, false>, dim3(x, blocks), kJoinThreads, 0, stream, true, p);

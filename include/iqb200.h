@@ -299,7 +299,9 @@ int iq_moe_down(const iq_moe_down_args* a, void* stream);
  * the caches ([capacity, kv_heads, head_dim], bf16 or e4m3; iq_qkv_heads writes them).
  * lengths[b] counts the rows, the new tokens' among them: row r of the step is at n - q_len +
  * r (n = lengths[b]) and sees the rows in (that - window, that], or all up to it with window
- * 0.  out = softmax(scale q.k) v per query head (q_heads / kv_heads of them share a key/value
+ * 0.  The window counts rows, so it is one of tokens only while rows lie in the order of their
+ * tokens: not after iq_kv_evict has cut the sequence, which fills freed rows with later ones.
+ * out = softmax(scale q.k) v per query head (q_heads / kv_heads of them share a key/value
  * head), lse = log of the softmax's sum; a row that sees nothing (a sequence of fewer than
  * q_len rows, an empty one) gets zeros and -infinity.  Rows outside a query row's view never
  * reach it, infinities and NaNs there included, nor do rows past lengths[b].  Softmax
@@ -359,7 +361,8 @@ int iq_attn_decode(const iq_attn_args* a, void* stream);
  * (position < keep_first, or >= seen[b] - keep_last), then those of the largest weight, ties
  * to the lower row (a NaN weight counts as the lowest).  The rows that stay and lie below
  * `budget` keep their place; the others move into the freed places below it, the i-th such
- * row (ascending) into the i-th place.  K and V move in place; weights and positions of the
+ * row (ascending) into the i-th place.  From then on rows do not lie in the order of their
+ * tokens (positions has it), so iq_attn_decode's window no longer means one.  K and V move in place; weights and positions of the
  * rows that stay go to weights_out / positions_out (which may be weights / positions
  * themselves, with their strides, but share no memory with them otherwise), entries from `budget` (or n) on are left as they were; lengths_out[b] = min(n,
  * budget) (not in the memory of `lengths` or `seen`: every head reads those).  Sequences must not share pages.

@@ -117,13 +117,17 @@ class PagedKvCache:
 class PagedAttention:
     """Attention of a step's rows over a `PagedKvCache`: q `[batch * q_len, q_heads, D]` (what
     `PrologueKernels` returns) -> `[batch * q_len, q_heads * D]` bf16 (what `OProjGemv` takes),
-    in one arena slot.  `window` > 0: sliding-window attention."""
+    in one arena slot.  `window` > 0: sliding-window attention, over a cache without a budget
+    only: the window counts rows, and eviction gives up their order."""
 
     def __init__(self, q_heads: int, cache: PagedKvCache, *, ws, window: int = 0, scale=None):
         if q_heads % cache.kv_heads:
             raise ValueError(f"{q_heads} query heads do not share {cache.kv_heads} key/value heads")
         if window < 0:
             raise ValueError(f"window must not be negative, got {window}")
+        if window and cache.budget is not None:
+            raise ValueError("a sliding window needs a cache without a budget: eviction does not "
+                             "keep the rows in the order of their tokens")
         self.q_heads, self.cache, self.window, self.scale = q_heads, cache, window, scale
         rows, d = cache.batch * cache.q_len, cache.head_dim
         self.out = ws.slot(("attention", "out"), (rows, q_heads * d), torch.bfloat16)

@@ -171,8 +171,8 @@ class DecodeSlice:
     i+1's attention norm) is what layer i+1's QKV product reads.
 
     With `kv` (a `PagedKvCache` of as many layers; batch x q_len is the slice's `q_len`) the
-    attention runs between the two, over that cache (`window` > 0: sliding-window), the
-    step's rows, positions and rotary angles come from the cache's own counters
+    attention runs between the two, over that cache (`window` > 0: sliding-window, for a cache
+    without a budget), the step's rows, positions and rotary angles come from the cache's own counters
     (`max_positions` bounds them), and sequences past the cache's budget are cut at the end
     of the step: a captured step decodes the next token each time it is replayed.  Without
     `kv` the attention output `ao` is a stand-in the caller supplies per layer, and the

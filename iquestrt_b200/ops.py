@@ -497,8 +497,9 @@ def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, sca
     `k_cache` / `v_cache [capacity, kv_heads, D]` are what `qkv_heads` writes (bf16 or e4m3),
     row j of sequence b being row `page_table[b, j // page_size] * page_size + j % page_size`;
     `lengths [batch]` (int32) counts the rows with the new ones.  New token r sees the rows up
-    to its own, the last `window` of them if `window` is not 0.  A token that sees nothing
-    gets zeros, and -inf in `lse [batch, q_len, q_heads]` (fp32, optional).  `scale` defaults
+    to its own, the last `window` of them if `window` is not 0: rows of the cache, whose order
+    is that of the tokens until `kv_evict` cuts the sequence, so not for such a cache.  A token
+    that sees nothing gets zeros, and -inf in `lse [batch, q_len, q_heads]` (fp32, optional).  `scale` defaults
     to D ** -0.5.
 
     `weights [batch, kv_heads, >= rows]` (fp32) gains each row's softmax weights, summed over
@@ -588,7 +589,8 @@ def kv_evict(k_cache, v_cache, page_table, lengths, weights, positions, seen, *,
     and in ascending order, into the places freed there, with their weights and positions
     (`weights_out` / `positions_out`, by default the inputs themselves).  `lengths_out [batch]`
     (int32, not in the memory of `lengths` or `seen`: layers of a model share the lengths of
-    before) gets the new lengths.  Sequences must not share pages."""
+    before) gets the new lengths.  Sequences must not share pages.  The rows' order is given up
+    with that (`positions` keeps it): a window of `attn_decode` would count the wrong rows."""
     if not isinstance(weights, torch.Tensor) or weights.dim() != 3:
         raise ValueError("weights must be a tensor [batch, kv_heads, rows]")
     shape, index = weights.shape, weights.get_device()

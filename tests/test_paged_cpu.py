@@ -291,3 +291,24 @@ def test_holders_refuse():
         PagedAttention(3, kv, ws=ws)
     with pytest.raises(ValueError, match="window"):
         PagedAttention(4, kv, ws=ws, window=-1)
+
+
+def test_a_window_over_a_cache_that_evicts_is_refused():
+    """Eviction fills freed rows with later ones, so the last rows are not the last tokens: five
+    rows cut to four (row 1 has the least weight) leave token 4 in row 1, and the next token's
+    window of two rows would see rows 3 and 4, tokens 3 and 5, instead of tokens 4 and 5."""
+    from iquestrt_b200.kernels import PagedAttention, PagedKvCache
+    from iquestrt_b200.workspace import Workspace
+    pos = torch.arange(6, dtype=torch.int32).view(1, 1, 6)
+    w = torch.tensor([[[5.0, 0.0, 3.0, 2.0, 1.0, 0.0]]])
+    kv = torch.zeros(6, 1, 2)
+    moved = P.kv_evict(kv, kv, torch.arange(6)[None], torch.tensor([5]), w, pos, torch.tensor([5]),
+                       1, budget=4)[3]
+    assert moved[0, 0, :4].tolist() == [0, 4, 2, 3]
+    cache = PagedKvCache(1, 1, 1, 128, rows=64, page_size=16, budget=24, device="cpu")
+    ws = Workspace(device="cpu")
+    for window in (1, 8, 1000):
+        with pytest.raises(ValueError, match="without a budget"):
+            PagedAttention(4, cache, ws=ws, window=window)
+    PagedAttention(4, cache, ws=ws)
+    PagedAttention(4, PagedKvCache(1, 1, 1, 128, rows=64, page_size=16, device="cpu"), ws=ws, window=8)

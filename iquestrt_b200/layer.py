@@ -24,6 +24,7 @@ from __future__ import annotations
 import torch
 
 from . import ops
+from ._lib import IqError
 from .kernels import (MoeDecodeKernels, MultimemARTail, MultimemMLPTail, OProjGemv, PagedAttention,
                       PagedKvCache, PrologueKernels, RouterSelect, TailKernels)
 from .synth import HEADS, HeadShape, LayerShape, rope_tables
@@ -264,7 +265,12 @@ class DecodeSlice:
         return 8 if self.kv.budget is None else 10
 
     def check(self) -> None:
+        """Synchronises and raises if any launch recorded a device-side error, those over the
+        KV cache among them (they report to the cache's scratch, the others to the layer's)."""
+        code = 0 if self.kv is None else self.kv.scratch.status()
         self.layer.check()
+        if code:
+            raise IqError("paged KV cache", code)
 
 
 class HostSliceStep:

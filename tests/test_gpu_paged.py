@@ -590,3 +590,48 @@ def test_decode_slice_over_a_paged_cache(budget):
     sl.check()
     graphed.check()
     assert sl.kv.scratch.status() == 0
+
+
+def _slices(kv_heads=2, q_heads=8, layers=2, q_len=2, batch=2, **kv_args):
+    """A maker of equal small slices over paged caches with the same prompts' rows in them."""
+    from iquestrt_b200 import synth
+    from iquestrt_b200.kernels import PagedKvCache
+    from iquestrt_b200.layer import DecodeSlice
+    shape = synth.LayerShape(hidden=1024, q_dim=128 * q_heads, n_experts=16, top_k=2, inter=256)
+    heads = synth.HeadShape(q_heads=q_heads, kv_heads=kv_heads)
+    weights = [(synth.make_layer(shape, device=DEV, seed=9, layer=i),
+                synth.make_prologue(shape, heads, device=DEV, seed=9, layer=i))
+               for i in range(layers)]
+
+    def make(window=0, max_positions=200):
+        kv = PagedKvCache(layers, batch, kv_heads, 128, q_len=q_len // batch,
+                          **{**dict(rows=64, page_size=16), **kv_args})
+        g = _gen(95)
+        for x in kv.k + kv.v:
+            x.copy_(torch.randn(x.shape, generator=g, device=DEV))
+        return DecodeSlice(shape, weights, heads=heads, q_len=q_len, kv=kv, window=window,
+                           max_positions=max_positions)
+
+    def inputs(i):
+        g = _gen(1000 + i)
+        return tuple(torch.randn(q_len, 1024, generator=g, device=DEV).to(BF16) for _ in range(2))
+
+    return make, inputs
+
+
+def test_slice_check_sees_errors_over_the_cache():
+    """A page outside the cache, below the rows that the step writes: attention reads zeros there
+    and says so, and so does the slice."""
+    from iquestrt_b200._lib import IqError
+    make, inputs = _slices()
+    sl = make()
+    sl.kv.set_lengths([33, 5])
+    sl.step(*inputs(0))
+    sl.check()
+    sl.kv.page_table[0, 0] = sl.kv.capacity // 16
+    sl.step(*inputs(1))
+    with pytest.raises(IqError, match="paged KV cache"):
+        sl.check()
+    sl.kv.page_table[0, 0] = 0
+    sl.step(*inputs(2))
+    sl.check()

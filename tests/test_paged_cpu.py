@@ -312,3 +312,36 @@ def test_a_window_over_a_cache_that_evicts_is_refused():
             PagedAttention(4, cache, ws=ws, window=window)
     PagedAttention(4, cache, ws=ws)
     PagedAttention(4, PagedKvCache(1, 1, 1, 128, rows=64, page_size=16, device="cpu"), ws=ws, window=8)
+
+
+@pytest.mark.parametrize("layer_code,cache_code", [(0, 0), (0, 5), (5, 0), (5, 3)])
+def test_slice_check_reads_the_caches_status_too(layer_code, cache_code):
+    """The attention, eviction and bookkeeping of a slice report to the cache's scratch: an error
+    there is the slice's, and is not reported a second time."""
+    from types import SimpleNamespace
+
+    from iquestrt_b200._lib import IqError
+    from iquestrt_b200.layer import DecodeSlice
+
+    class Status:
+        def __init__(self, code):
+            self.code = code
+
+        def status(self):
+            code, self.code = self.code, 0
+            return code
+
+        def raise_on_error(self):
+            code = self.status()
+            if code:
+                raise IqError("fake", code)
+
+    sl = object.__new__(DecodeSlice)
+    sl.layer = SimpleNamespace(check=Status(layer_code).raise_on_error)
+    sl.kv = SimpleNamespace(scratch=Status(cache_code))
+    if layer_code or cache_code:
+        with pytest.raises(IqError):
+            sl.check()
+    sl.check()
+    sl.kv = None
+    sl.check()

@@ -81,18 +81,60 @@ class PagedKvCache:
             self._scratch = ops.default_scratch(self.held.device)
         return self._scratch
 
-    def set_lengths(self, lengths, seen=None) -> None:
+    def set_lengths(self, lengths, seen=None, *, positions=None, weights=None) -> None:
         """Declares the rows already written (a prompt's) per sequence, and the tokens seen (as
-        many, where nothing was evicted before).  Between steps only."""
-        n = torch.as_tensor(lengths, dtype=torch.int32)
+        many, where nothing was evicted before).  Between steps only.
+
+        With a budget the rows' positions and accumulated weights start anew: `positions` and
+        `weights` are a tensor `[batch, kv_heads, rows]` a layer (int32, fp32; fewer rows will do
+        if they hold the longest sequence).  Without `positions` row j is token j, which is so
+        only where nothing was evicted; without `weights` every row starts at 0, and of rows that
+        no step's attention has told apart the later go first.  The cache's own tensors
+        (`cache.positions`, `cache.weights`) say that they are filled already."""
+        n = torch.as_tensor(lengths, dtype=torch.int32).cpu()
         if n.shape != (self.batch,) or int(n.min()) < 0 or int(n.max()) > self.rows:
             raise ValueError(f"lengths must be [{self.batch}] within 0..{self.rows}, got "
                              f"{n.tolist()}")
+        s = n if seen is None else torch.as_tensor(seen, dtype=torch.int32).cpu()
+        if s.shape != (self.batch,) or bool((s < (0 if self.budget is None else n)).any()):
+            raise ValueError(f"seen must be [{self.batch}], not negative and (with a budget) no less "
+                             f"than the rows {n.tolist()}, got {s.tolist()}")
+        if self.budget is None:
+            if positions is not None or weights is not None:
+                raise ValueError("positions and weights are kept with a budget only")
+        else:
+            if positions is None and not torch.equal(s, n):
+                raise ValueError("sequences that have seen more tokens than they hold need their "
+                                 "rows' positions")
+            for name, given, kept in (("positions", positions, self.positions),
+                                      ("weights", weights, self.weights)):
+                self._check_state(name, given, kept, int(n.max()))
         self.held.copy_(n)
-        self.seen.copy_(n if seen is None else torch.as_tensor(seen, dtype=torch.int32))
-        if self.weights is not None and seen is None:
-            for p in self.positions:
-                p.copy_(torch.arange(self.rows, dtype=torch.int32, device=p.device).expand_as(p))
+        self.seen.copy_(s)
+        if self.budget is None:
+            return
+        order = torch.arange(self.rows, dtype=torch.int32, device=self.held.device)
+        for i, (p, w) in enumerate(zip(self.positions, self.weights)):
+            if positions is None:
+                p.copy_(order.expand_as(p))
+            elif positions[i] is not p:
+                p[..., :positions[i].shape[2]].copy_(positions[i])
+            if weights is None:
+                w.zero_()
+            elif weights[i] is not w:
+                w[..., :weights[i].shape[2]].copy_(weights[i])
+
+    def _check_state(self, name, given, kept, longest) -> None:
+        if given is None:
+            return
+        if len(given) != len(kept):
+            raise ValueError(f"{name} must be a tensor for each of {len(kept)} layers, got {len(given)}")
+        for x in given:
+            if not isinstance(x, torch.Tensor) or x.dtype != kept[0].dtype or x.dim() != 3 \
+                    or x.shape[:2] != kept[0].shape[:2] or not longest <= x.shape[2] <= self.rows:
+                what = f"{tuple(x.shape)} {x.dtype}" if isinstance(x, torch.Tensor) else type(x)
+                raise ValueError(f"{name} must be [{self.batch}, {self.kv_heads}, {longest}.."
+                                 f"{self.rows}] {kept[0].dtype} tensors, got {what}")
 
     def advance(self, *, max_positions: int = 0, pdl: bool = False) -> None:
         """Rows and positions of the step's tokens into `slot` / `pos`; `lengths` and `seen`

@@ -635,3 +635,33 @@ def test_slice_check_sees_errors_over_the_cache():
     sl.kv.page_table[0, 0] = 0
     sl.step(*inputs(2))
     sl.check()
+
+
+def test_a_reused_cache_is_as_a_fresh_one():
+    """Second prompts in a cache that has decoded and evicted before: every step past the budget
+    as with a cache of their own, bit for bit."""
+    make, inputs = _slices(budget=40, keep_first=2, keep_last=10)
+    used, fresh = make(), make()
+    used.kv.set_lengths([39, 12])
+    for i in range(8):
+        used.step(*inputs(50 + i))
+    used.check()
+    for a, b in zip(used.kv.k + used.kv.v, fresh.kv.k + fresh.kv.v):
+        a.copy_(b)
+    for sl in (used, fresh):
+        sl.kv.set_lengths([36, 40])
+    for i in range(8):
+        got = [x.clone() for x in used.step(*inputs(i))]
+        want = fresh.step(*inputs(i))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        held = fresh.kv.held.tolist()
+        assert used.kv.held.tolist() == held == [min(40, 37 + i), 40]
+        for layer in range(2):
+            for name in ("k", "v"):
+                assert torch.equal(_bits(getattr(used.kv, name)[layer]), _bits(getattr(fresh.kv, name)[layer]))
+            for name in ("weights", "positions"):
+                for b, n in enumerate(held):
+                    a, c = (getattr(sl.kv, name)[layer][b, :, :n] for sl in (used, fresh))
+                    assert torch.equal(_bits(a), _bits(c))
+    for sl in (used, fresh):
+        sl.check()

@@ -345,3 +345,77 @@ def test_slice_check_reads_the_caches_status_too(layer_code, cache_code):
     sl.check()
     sl.kv = None
     sl.check()
+
+
+def _budget_cache():
+    from iquestrt_b200.kernels import PagedKvCache
+    return PagedKvCache(2, 2, 3, 128, rows=64, page_size=16, budget=40, device="cpu")
+
+
+def test_set_lengths_starts_the_bookkeeping_anew():
+    """Nothing of the sequences that a cache held before is left: weights, positions, counts."""
+    fresh, used = _budget_cache(), _budget_cache()
+    for x in used.weights:
+        x.fill_(5.0)
+    for x in used.positions:
+        x.fill_(-9)
+    used.held.fill_(17)
+    used.seen.fill_(18)
+    for kv in (fresh, used):
+        kv.set_lengths([33, 5])
+        assert kv.held.tolist() == kv.seen.tolist() == [33, 5]
+    for name in ("weights", "positions"):
+        for a, b in zip(getattr(fresh, name), getattr(used, name)):
+            assert torch.equal(a, b)
+    assert float(used.weights[0].abs().sum()) == 0
+    assert torch.equal(used.positions[1][1, 2], torch.arange(64, dtype=torch.int32))
+
+
+def test_set_lengths_takes_a_prompts_weights_and_positions():
+    kv = _budget_cache()
+    g = torch.Generator().manual_seed(3)
+    w = [torch.rand(2, 3, 40, generator=g) for _ in range(2)]
+    pos = [torch.randint(0, 90, (2, 3, 64), generator=g, dtype=torch.int32) for _ in range(2)]
+    kv.set_lengths([33, 40], seen=[90, 100], positions=pos, weights=w)
+    assert kv.held.tolist() == [33, 40] and kv.seen.tolist() == [90, 100]
+    for i in range(2):
+        assert torch.equal(kv.weights[i][..., :40], w[i]) and torch.equal(kv.positions[i], pos[i])
+    # the cache's own: filled already, and left as they are
+    kept = [x.clone() for x in kv.weights + kv.positions]
+    kv.set_lengths(torch.tensor([30, 1]), torch.tensor([95, 1]), positions=kv.positions,
+                   weights=kv.weights)
+    assert all(torch.equal(a, b) for a, b in zip(kept, kv.weights + kv.positions))
+    assert kv.held.tolist() == [30, 1] and kv.seen.tolist() == [95, 1]
+    # seen as many as held: nothing was evicted
+    kv.set_lengths([30, 1], [30, 1])
+    assert kv.positions[0][1, 0].tolist() == list(range(64)) and float(kv.weights[1].sum()) == 0
+
+
+@pytest.mark.parametrize("change,message", [
+    (dict(seen=[90]), "seen"), (dict(seen=90), "seen"), (dict(seen=[90, -1]), "seen"),
+    (dict(seen=[32, 5]), "seen"), (dict(seen=[90, 5]), "positions"),
+    (dict(positions=[torch.zeros(2, 3, 64, dtype=torch.int32)]), "2 layers"),
+    (dict(positions=[torch.zeros(2, 3, 32, dtype=torch.int32)] * 2), "33..64"),
+    (dict(positions=[torch.zeros(2, 3, 65, dtype=torch.int32)] * 2), "33..64"),
+    (dict(positions=[torch.zeros(2, 3, 64)] * 2), "int32"),
+    (dict(weights=[torch.zeros(2, 2, 64)] * 2), "weights"),
+    (dict(weights=torch.zeros(2, 64)), "weights"),
+])
+def test_set_lengths_refuses(change, message):
+    """And changes nothing where it refuses."""
+    kv = _budget_cache()
+    kv.weights[0].fill_(2.0)
+    with pytest.raises(ValueError, match=message):
+        kv.set_lengths([33, 5], **change)
+    assert kv.held.tolist() == kv.seen.tolist() == [0, 0] and float(kv.weights[0].min()) == 2.0
+
+
+def test_set_lengths_without_a_budget():
+    """Positions are the rotary embedding's alone: any count that is not negative will do."""
+    from iquestrt_b200.kernels import PagedKvCache
+    kv = PagedKvCache(1, 2, 1, 128, rows=64, page_size=16, device="cpu")
+    kv.set_lengths([3, 64], seen=[0, 700])
+    assert kv.held.tolist() == [3, 64] and kv.seen.tolist() == [0, 700]
+    for change, message in ((dict(seen=[-1, 3]), "seen"), (dict(weights=[torch.zeros(2, 1, 64)]), "budget")):
+        with pytest.raises(ValueError, match=message):
+            kv.set_lengths([3, 64], **change)

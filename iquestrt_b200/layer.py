@@ -279,13 +279,17 @@ class HostSliceStep:
     launches, and the copy of the last layer's output back to pinned host memory (`HostStep`
     for the slice).  The stand-in attention outputs `aos` stay on the device, where an
     attention kernel would have written them (None for a slice with a KV cache; building this
-    object then takes one step).  Captures the slice's CURRENT `layers`."""
+    object then takes one step).  What the caller's current stream has been given before a call
+    (a prompt's rows, `set_lengths`) is done before the step.  Captures the slice's CURRENT
+    `layers`."""
 
     def __init__(self, sl: DecodeSlice, aos=None, *, pdl: bool = True):
         layer = sl.layer
         dev = layer.norm_out.device
         q, h = layer.q_len, layer.shape.hidden
+        self._over_cache = sl.kv is not None
         self.stream = torch.cuda.Stream(device=dev)
+        self.stream.wait_stream(torch.cuda.current_stream(dev))
         self.res_pin = torch.zeros(q, h, dtype=torch.bfloat16).pin_memory()
         self.xn_pin = torch.zeros(q, h, dtype=torch.bfloat16).pin_memory()
         self.out_pin = torch.empty(q, h, dtype=torch.bfloat16).pin_memory()
@@ -312,6 +316,8 @@ class HostSliceStep:
     def __call__(self, residual_host, xn_host):
         self.res_pin.copy_(residual_host)
         self.xn_pin.copy_(xn_host)
+        if self._over_cache:
+            self.stream.wait_stream(torch.cuda.current_stream(self.stream.device))
         with torch.cuda.stream(self.stream):
             self.graph.replay()
         self.stream.synchronize()

@@ -665,3 +665,31 @@ def test_a_reused_cache_is_as_a_fresh_one():
                     assert torch.equal(_bits(a), _bits(c))
     for sl in (used, fresh):
         sl.check()
+
+
+def test_host_step_waits_for_the_callers_stream():
+    """A prompt's rows that the caller's stream is still writing when the step is called: the
+    step attends over them, as a step on that stream does."""
+    from iquestrt_b200.layer import HostSliceStep
+    make, inputs = _slices()
+    on_stream, from_host = make(), make()
+    host = HostSliceStep(from_host)
+    g = _gen(97)
+    prompt = [torch.randn(x.shape, generator=g, device=DEV).to(x.dtype) for x in on_stream.kv.k]
+
+    def write(kv, rows):
+        for k, v, x in zip(kv.k, kv.v, rows):
+            k.copy_(x)
+            v.copy_(x)
+
+    on_stream.kv.set_lengths([33, 5])
+    write(on_stream.kv, prompt)
+    want = on_stream.step(*inputs(0))[0].cpu()
+    res, xn = (x.cpu() for x in inputs(0))
+    from_host.kv.set_lengths([33, 5])
+    write(from_host.kv, [torch.zeros_like(x) for x in prompt])
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)               # some 50 ms
+    write(from_host.kv, prompt)
+    assert torch.equal(host(res, xn), want)
+    from_host.check()

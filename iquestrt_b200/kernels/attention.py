@@ -4,6 +4,8 @@ and lengths, attends, and (with a budget) evicts, so that replaying it decodes t
 token.  The reference's counterpart is its online split-KV attention over flat caches and
 sliding-window rings (iquestrt/kernels/attention.py:40-57, iquestrt/kv.py:57-66)."""
 
+import contextlib
+
 import torch
 
 from .. import ops
@@ -135,6 +137,29 @@ class PagedKvCache:
                 what = f"{tuple(x.shape)} {x.dtype}" if isinstance(x, torch.Tensor) else type(x)
                 raise ValueError(f"{name} must be [{self.batch}, {self.kv_heads}, {longest}.."
                                  f"{self.rows}] {kept[0].dtype} tensors, got {what}")
+
+    @contextlib.contextmanager
+    def rehearsal(self):
+        """What runs inside, on the current stream, leaves the cache as it was: the warm-up step
+        before a capture.  The sequences hold nothing meanwhile, and the rows of the steps' first
+        tokens are the caches' first ones for all of them, so that these rows are all there is
+        to put back (sequences that overwrite one another's change nothing but these)."""
+        table = self.page_table
+        rows = min(self.q_len, self.page_size, self.capacity)
+        kept = [self.held, self.lengths, self.seen, self.slot, self.pos]
+        kept += [x[:rows] for x in self.k + self.v]
+        if self.budget is not None:
+            kept += [x[..., :self.q_len] for x in self.weights + self.positions]
+        was = [x.clone() for x in kept]
+        self.page_table = torch.zeros_like(table)
+        self.held.zero_()
+        self.seen.zero_()
+        try:
+            yield self
+        finally:
+            self.page_table = table
+            for x, y in zip(kept, was):
+                x.copy_(y)
 
     def advance(self, *, max_positions: int = 0, pdl: bool = False) -> None:
         """Rows and positions of the step's tokens into `slot` / `pos`; `lengths` and `seen`

@@ -21,6 +21,8 @@ CTAs of the same launch) or "pull" (signal, wait, `multimem.ld_reduce` on the la
 
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import ops
@@ -278,8 +280,8 @@ class HostSliceStep:
     the stream entering layer 0 and its norm from pinned host memory, every layer's
     launches, and the copy of the last layer's output back to pinned host memory (`HostStep`
     for the slice).  The stand-in attention outputs `aos` stay on the device, where an
-    attention kernel would have written them (None for a slice with a KV cache; building this
-    object then takes one step).  What the caller's current stream has been given before a call
+    attention kernel would have written them (None for a slice with a KV cache, which building
+    this object leaves as it was).  What the caller's current stream has been given before a call
     (a prompt's rows, `set_lengths`) is done before the step.  Captures the slice's CURRENT
     `layers`."""
 
@@ -303,7 +305,8 @@ class HostSliceStep:
             self.out_pin.copy_(out, non_blocking=True)
 
         with torch.cuda.stream(self.stream):
-            body()
+            with sl.kv.rehearsal() if self._over_cache else contextlib.nullcontext():
+                body()
             self.stream.synchronize()
             sl.check()
             self.graph = torch.cuda.CUDAGraph()

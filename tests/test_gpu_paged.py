@@ -693,3 +693,46 @@ def test_host_step_waits_for_the_callers_stream():
     write(from_host.kv, prompt)
     assert torch.equal(host(res, xn), want)
     from_host.check()
+
+
+@pytest.mark.parametrize("kv_args", [
+    dict(), dict(budget=40, keep_first=2, keep_last=10),
+    dict(q_len=8, page_size=1, budget=2, keep_first=0),      # more new rows than the budget
+    dict(q_len=6, page_size=4, rows=16)], ids=["plain", "budget", "small", "tight"])
+def test_host_steps_over_a_cache(kv_args):
+    """Building a host step leaves the cache as it was, a full budget's rows among it; its steps
+    are those of a slice that is called step by step, bit for bit."""
+    from iquestrt_b200.layer import HostSliceStep
+    make, inputs = _slices(**kv_args)
+    sl, other = make(), make()
+    full = kv_args.get("budget") or 7
+    g = _gen(98)
+    w = None
+    if sl.kv.budget is not None:
+        w = [torch.rand(x.shape, generator=g, device=DEV) for x in sl.kv.weights]
+    for s in (sl, other):
+        s.kv.set_lengths([full, 1], weights=w)
+    names = ("held", "lengths", "seen", "slot", "pos", "page_table", "k", "v", "weights", "positions")
+
+    def state(kv):
+        parts = [getattr(kv, n) for n in names]
+        return [x.clone() for part in parts if part is not None
+                for x in (part if isinstance(part, list) else [part])]
+
+    before = state(sl.kv)
+    host = HostSliceStep(sl)
+    assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip(before, state(sl.kv)))
+    for i in range(3):
+        res, xn = (x.cpu() for x in inputs(i))
+        got = host(res, xn).clone()
+        assert torch.equal(got, other.step(*inputs(i))[0].cpu())
+        assert sl.kv.held.tolist() == other.kv.held.tolist()
+        assert sl.kv.seen.tolist() == other.kv.seen.tolist()
+        for a, b in zip(sl.kv.k + sl.kv.v, other.kv.k + other.kv.v):
+            assert torch.equal(_bits(a), _bits(b))
+        for b, n in enumerate(sl.kv.held.tolist()):
+            for a, c in zip((sl.kv.weights or []) + (sl.kv.positions or []),
+                            (other.kv.weights or []) + (other.kv.positions or [])):
+                assert torch.equal(_bits(a[b, :, :n]), _bits(c[b, :, :n]))
+    sl.check()
+    other.check()

@@ -419,3 +419,40 @@ def test_set_lengths_without_a_budget():
     for change, message in ((dict(seen=[-1, 3]), "seen"), (dict(weights=[torch.zeros(2, 1, 64)]), "budget")):
         with pytest.raises(ValueError, match=message):
             kv.set_lengths([3, 64], **change)
+
+
+@pytest.mark.parametrize("budget,page", [(None, 16), (40, 16), (1, 2)])
+def test_rehearsal_puts_back_what_a_step_writes(budget, page):
+    """A step's writes (rows, weights and positions of the first tokens, counts) are undone, also
+    when the step fails; the page table is the cache's own again."""
+    from iquestrt_b200.kernels import PagedKvCache
+    kv = PagedKvCache(2, 2, 3, 16, rows=64, q_len=3, page_size=page, budget=budget, device="cpu",
+                      keep_first=0, dtype=torch.bfloat16)
+    kv.set_lengths([33, 5])
+    g = torch.Generator().manual_seed(5)
+    for x in kv.k + kv.v + (kv.weights or []):
+        x.copy_(torch.rand(x.shape, generator=g))
+
+    def state():
+        return [x.clone() for x in [kv.held, kv.lengths, kv.seen, kv.slot, kv.pos, kv.page_table,
+                                    *kv.k, *kv.v, *(kv.weights or []), *(kv.positions or [])]]
+
+    before, table = state(), kv.page_table
+    for fail in (False, True):
+        try:
+            with kv.rehearsal():
+                assert kv.held.tolist() == kv.seen.tolist() == [0, 0]
+                for b in range(2):
+                    rows = P.rows_of(kv.page_table, b, 3, page)
+                    for x in kv.k + kv.v:
+                        x[rows] = 7.0
+                for x in (kv.weights or []) + (kv.positions or []):
+                    x[..., :3] = 9
+                for x in (kv.held, kv.lengths, kv.seen, kv.slot, kv.pos):
+                    x.fill_(3)
+                if fail:
+                    raise ArithmeticError
+        except ArithmeticError:
+            assert fail
+        assert kv.page_table is table
+        assert all(torch.equal(a, b) for a, b in zip(before, state()))

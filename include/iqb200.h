@@ -319,8 +319,8 @@ int iq_moe_down(const iq_moe_down_args* a, void* stream);
  * * q_len up to 512.  Strides are in elements; those of the caches, q and out times the
  * element size, and their addresses, are multiples of 16 bytes.  `work` (iq_attn_work_bytes, 16-byte
  * aligned) needs no initialisation; calls that share it must be ordered.  A length outside
- * the page table is clamped and a page outside the cache read as zeros, with IQ_ERR_ROUTE in
- * the status word. */
+ * the page table is clamped and a row outside the cache (its page, or the end of a page that
+ * straddles the cache's) read as zeros, with IQ_ERR_ROUTE in the status word. */
 typedef struct iq_attn_args {
   const void* q;            /* bf16 [batch, q_len, q_heads, head_dim] */
   int64_t q_b, q_r, q_h;

@@ -525,13 +525,15 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
       }
       if (lane < copies) {
         // a box without keys of the unit, or of a page outside the cache, is read past the
-        // cache's end, which fills it with zeros
+        // cache's end, which fills it with zeros; so are the last rows of a page that straddles
+        // that end
         const int j = ld.j + key;
         int at = p.pages.capacity;
         if (j < ld.n && j + p.box_rows > ld.lo) {
           const int row = page_row(p.pages, id_next, j);
           if (row >= 0) at = row;
-          else if (p.status) atomicCAS(p.status, 0, IQ_ERR_ROUTE);
+          if (p.pages.capacity - at < min(p.box_rows, ld.n - j) && p.status)
+            atomicCAS(p.status, 0, IQ_ERR_ROUTE);
         }
         tma_3d_g2s(dst + stage * G::STAGE, map, x * G::PITCH, at, ld.h0 + head,
                    bar_full + kgr * G::MAX_STAGES + stage);

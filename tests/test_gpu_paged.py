@@ -736,3 +736,28 @@ def test_host_steps_over_a_cache(kv_args):
                 assert torch.equal(_bits(a[b, :, :n]), _bits(c[b, :, :n]))
     sl.check()
     other.check()
+
+
+@pytest.mark.parametrize("kv", [E4M3, BF16], ids=["e4m3", "bf16"])
+@pytest.mark.parametrize("page,cut", [(64, 1), (64, 40), (24, 5), (3, 1), (256, 200)])
+def test_a_page_that_straddles_the_caches_end(scratch, kv, page, cut):
+    """A cache whose rows are no whole number of pages: up to its last row all is well; a row
+    behind it is read as zeros and the status says so, whether pages are copied in boxes or
+    gathered row by row."""
+    from iquestrt_b200 import ops
+    g = _gen(71)
+    table = torch.randperm(10, generator=g, device=DEV).int().view(2, 5)
+    table = torch.where(table == table[0, 4], 10, table)     # sequence 0 ends in the last page
+    capacity = 11 * page - cut
+    k = torch.zeros(11 * page, 2, 128, device=DEV)
+    v = torch.zeros_like(k)
+    k[:capacity] = torch.randn(capacity, 2, 128, generator=g, device=DEV)
+    v[:capacity] = torch.randn(capacity, 2, 128, generator=g, device=DEV)
+    k, v = k.to(kv), v.to(kv)
+    q = (2.5 * torch.randn(2, 2, 8, 128, generator=g, device=DEV)).to(BF16)
+    for over in (0, 1, cut):
+        lengths = [5 * page - cut + over, 4 * page]
+        n = torch.tensor(lengths, dtype=torch.int32, device=DEV)
+        out = ops.attn_decode(q, k[:capacity], v[:capacity], table, n, page_size=page, scratch=scratch)
+        assert scratch.status() == (5 if over else 0), over
+        _check(out, None, P.attn_decode(q, k, v, table, n, page), kv, 128, max(lengths))

@@ -313,7 +313,9 @@ int iq_moe_down(const iq_moe_down_args* a, void* stream);
  * With `weights`, weights[b][h][j] gains the sum of the softmax weights that the query heads
  * and rows of key/value head h gave row j; for the step's own rows it is set to it, and
  * positions[b][h][j] (where given) to seen[b] - n + j: `seen` counts the tokens sequence b
- * has seen in all, which eviction leaves larger than its length.
+ * has seen in all, which eviction leaves larger than its length.  With `slot` (what
+ * iq_kv_advance wrote) a sequence without room for the step's tokens, slot[b * q_len] < 0, is
+ * left out of both: its newest rows are not the step's, and its queries mean nothing.
  *
  * head_dim is a multiple of 16 up to 256, q_len 1..8, batch up to 1024, (q_heads / kv_heads)
  * * q_len up to 512.  Strides are in elements; those of the caches, q and out times the
@@ -345,6 +347,7 @@ typedef struct iq_attn_args {
   int* positions;           /* optional int32, same shape; with `seen` */
   int64_t p_b, p_h;
   const int* seen;          /* [batch] */
+  const int64_t* slot;      /* optional [batch * q_len]; with `weights` */
   void* work;
   size_t work_bytes;
   int* status;              /* optional device status word */

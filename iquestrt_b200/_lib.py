@@ -128,8 +128,8 @@ class AttnArgs(C.Structure):
         ("out", C.c_void_p), ("o_b", C.c_int64), ("o_r", C.c_int64), ("o_h", C.c_int64),
         ("lse", C.c_void_p), ("weights", C.c_void_p), ("w_b", C.c_int64), ("w_h", C.c_int64),
         ("weights_rows", C.c_int), ("positions", C.c_void_p), ("p_b", C.c_int64),
-        ("p_h", C.c_int64), ("seen", C.c_void_p), ("work", C.c_void_p), ("work_bytes", C.c_size_t),
-        ("status", C.c_void_p), ("pdl", C.c_int),
+        ("p_h", C.c_int64), ("seen", C.c_void_p), ("slot", C.c_void_p), ("work", C.c_void_p),
+        ("work_bytes", C.c_size_t), ("status", C.c_void_p), ("pdl", C.c_int),
     ]
 
 

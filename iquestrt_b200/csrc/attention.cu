@@ -80,6 +80,7 @@ struct AttnParams {
   int* positions;
   long long p_b, p_h;
   const int* seen;
+  const long long* slot;                         // of the step's rows, or null
   unsigned joins;                                // blocks along x that join
   unsigned weight_chunks, weight_blocks;         // blocks a (sequence, head)'s weights take; all of them
   int* status;
@@ -1140,7 +1141,8 @@ constexpr int kJoinParts = 160;                  // partial results of a unit, a
 // weights[b, h, j] += sum over the head's query rows of 2^(x_j - lse2): a thread a key, on the
 // scores the split kernel left behind (L2 holds most of them).  Each block works out the rows'
 // lse2 from the partial results for itself, so these blocks need not wait for those that join.
-// The step's own rows are set, not added to, and get their positions.  64 / 8 heads over 32768
+// The step's own rows are set, not added to, and get their positions; a sequence that had no room
+// for them (slot < 0) keeps its weights and positions.  64 / 8 heads over 32768
 // keys of e4m3: 26.6 us with the weights, 8 MB of scores written and read once more.
 constexpr int kWeightKeys = 1024;                // keys a block (512: 27.5 us; 81.9 over 128k, 1024 74.6)
 
@@ -1148,6 +1150,7 @@ template <class G>
 __device__ __forceinline__ void add_weights(const AttnParams& p, int chunk, int bh, float* z /* [512] */) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = bh / p.kv_heads, h = bh - b * p.kv_heads;
+  if (p.slot && __ldg(p.slot + static_cast<long long>(b) * p.q_len) < 0) return;
   const SeqSpan s = seq_span(clamp_length(p, b, false), p.q_len, p.window);
   const int from = max(s.lo, chunk * kWeightKeys), to = min(s.n, (chunk + 1) * kWeightKeys);
   if (from >= to) return;
@@ -1577,7 +1580,7 @@ extern "C" int iq_attn_decode(const iq_attn_args* a, void* stream) {
     return IQ_ERR_UNSUPPORTED;
   const bool weights = a->weights != nullptr;
   if (weights && a->weights_rows < rows) return IQ_ERR_ARG;
-  if ((a->positions != nullptr) != (a->seen != nullptr) || (a->positions && !weights))
+  if ((a->positions != nullptr) != (a->seen != nullptr) || ((a->positions || a->slot) && !weights))
     return IQ_ERR_ARG;
   const AttnWork w = attn_work(a->batch, a->q_len, a->q_heads, a->kv_heads, a->head_dim,
                                static_cast<int>(rows), weights);
@@ -1642,6 +1645,7 @@ extern "C" int iq_attn_decode(const iq_attn_args* a, void* stream) {
     p.positions = a->positions;
     p.p_b = a->p_b; p.p_h = a->p_h;
     p.seen = a->seen;
+    p.slot = reinterpret_cast<const long long*>(a->slot);
   }
   const bool bf16 = a->kv_kind == IQ_ACT_BF16, pdl = a->pdl != 0;
   int rc;

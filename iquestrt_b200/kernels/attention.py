@@ -164,9 +164,8 @@ class PagedKvCache:
     def advance(self, *, max_positions: int = 0, pdl: bool = False) -> None:
         """Rows and positions of the step's tokens into `slot` / `pos`; `lengths` and `seen`
         count them from here on.  A sequence without room for them (or that would reach
-        `max_positions`) keeps its rows and counts, and the scratch's status word says so; what
-        the step then computes for it means nothing, the accumulated weights and positions of
-        its newest rows included."""
+        `max_positions`) keeps its rows, counts, weights and positions, and the scratch's status
+        word says so; the step's outputs for it mean nothing."""
         ops.kv_advance(self.page_table, self.held, self.seen, self.slot, self.pos,
                        page_size=self.page_size, capacity=self.capacity, q_len=self.q_len,
                        max_positions=max_positions, lengths_out=self.lengths, scratch=self.scratch, pdl=pdl)
@@ -207,7 +206,8 @@ class PagedAttention:
         shape = (c.batch, c.q_len, self.q_heads, c.head_dim)
         more = {}
         if c.weights is not None:
-            more = dict(weights=c.weights[layer], positions=c.positions[layer], seen=c.seen)
+            more = dict(weights=c.weights[layer], positions=c.positions[layer], seen=c.seen,
+                        slot=c.slot)
         ops.attn_decode(q.view(shape), c.k[layer], c.v[layer], c.page_table, c.lengths,
                         page_size=c.page_size, scale=self.scale, window=self.window,
                         out=self.out.view(shape), work=self.work, scratch=c.scratch, pdl=pdl, **more)

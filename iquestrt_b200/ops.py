@@ -490,7 +490,7 @@ class AttnWork:
 
 def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, scale=None,
                 window: int = 0, out=None, lse=None, weights=None, positions=None, seen=None,
-                work: AttnWork | None = None, scratch: Scratch | None = None, pdl: bool = True):
+                slot=None, work: AttnWork | None = None, scratch: Scratch | None = None, pdl: bool = True):
     """Attention of the last `q_len` tokens of each sequence over its paged KV cache
     (`iq_attn_decode`): `q [batch, q_len, q_heads, D]` bf16 -> `out`, same shape.
 
@@ -505,7 +505,9 @@ def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, sca
     `weights [batch, kv_heads, >= rows]` (fp32) gains each row's softmax weights, summed over
     the query heads of its key/value head and the new tokens; the new tokens' own entries are
     set, and those of `positions` (int32, same shape) to the tokens' positions, `seen [batch]`
-    (int32) being the tokens seen so far with the new ones.  Without `work` one is allocated
+    (int32) being the tokens seen so far with the new ones.  With `slot [batch * q_len]` (int64,
+    what `kv_advance` wrote) a sequence that had no room for the new tokens (slots of -1) keeps
+    its weights and positions; what its rows of `out` hold means nothing.  Without `work` one is allocated
     for the call.  A length or page out of range shows in `scratch`'s status word.  `pdl` lets
     the launch's set-up overlap the kernel before it; nothing is read or written before that
     kernel is done.
@@ -526,7 +528,7 @@ def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, sca
     if out is None:
         out = torch.empty(shape, dtype=_BF16, device=q.device)
     os_ = _take_out("out", out, _BF16, shape, index)
-    lse_ptr = w_ptr = pos_ptr = seen_ptr = w_rows = 0
+    lse_ptr = w_ptr = pos_ptr = seen_ptr = slot_ptr = w_rows = 0
     ws = ps = (0, 0)
     if lse is not None:
         _take("lse", lse, _F32, shape[:3], index)
@@ -546,6 +548,11 @@ def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, sca
         ps = _take_out("positions", positions, _I32, weights.shape, index)
         _take("seen", seen, _I32, (batch,), index)
         pos_ptr, seen_ptr = positions.data_ptr(), seen.data_ptr()
+    if slot is not None:
+        if weights is None:
+            raise ValueError("slot comes with weights")
+        _take("slot", slot, _I64, (batch * q_len,), index)
+        slot_ptr = slot.data_ptr()
     _gpu("q", index)
     if work is None:
         work = AttnWork(batch=batch, q_len=q_len, q_heads=q_heads, kv_heads=kv_heads, head_dim=d,
@@ -557,7 +564,7 @@ def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, sca
         ks[0], ks[1], vs[0], vs[1], kind, capacity, page_table.data_ptr(), ts, page_size, pages,
         lengths.data_ptr(), batch, q_len, q_heads, kv_heads, d, window,
         d ** -0.5 if scale is None else scale, out.data_ptr(), os_[0], os_[1], os_[2], lse_ptr,
-        w_ptr, ws[0], ws[1], w_rows, pos_ptr, ps[0], ps[1], seen_ptr, work.ptr, work.bytes,
+        w_ptr, ws[0], ws[1], w_rows, pos_ptr, ps[0], ps[1], seen_ptr, slot_ptr, work.ptr, work.bytes,
         0 if scratch is None else scratch.ptr, int(pdl)))
     return out
 

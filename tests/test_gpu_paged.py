@@ -761,3 +761,58 @@ def test_a_page_that_straddles_the_caches_end(scratch, kv, page, cut):
         out = ops.attn_decode(q, k[:capacity], v[:capacity], table, n, page_size=page, scratch=scratch)
         assert scratch.status() == (5 if over else 0), over
         _check(out, None, P.attn_decode(q, k, v, table, n, page), kv, 128, max(lengths))
+
+
+@pytest.mark.parametrize("q_len", [1, 3])
+def test_a_sequence_without_room_keeps_its_weights(scratch, q_len):
+    """Slots of -1: the sequence's weights and positions stay, the others' are what they are
+    without slots, bit for bit."""
+    from iquestrt_b200 import ops
+    page, kh = 16, 2
+    q, k, v, table, n = _case([700, 1500, 40], q_len, 8, kh, 128, E4M3, page, seed=14)
+    g = _gen(15)
+    w = torch.rand(3, kh, table.shape[1] * page, generator=g, device=DEV)
+    pos = torch.randint(0, 99, w.shape, generator=g, device=DEV, dtype=torch.int32)
+    slot = torch.arange(3 * q_len, device=DEV)
+    slot.view(3, q_len)[1] = -1
+    got = []
+    for more in (dict(), dict(slot=slot)):
+        ww, pp = w.clone(), pos.clone()
+        out = ops.attn_decode(q, k, v, table, n, page_size=page, weights=ww, positions=pp, seen=n + 9,
+                              scratch=scratch, **more)
+        got.append((out, ww, pp))
+    assert scratch.status() == 0
+    (out, ww, pp), (out2, ww2, pp2) = got
+    assert torch.equal(out, out2)
+    for b in (0, 2):
+        assert torch.equal(ww[b], ww2[b]) and torch.equal(pp[b], pp2[b])
+    assert torch.equal(ww2[1], w[1]) and torch.equal(pp2[1], pos[1])
+    assert not torch.equal(ww[1], w[1]) and not torch.equal(pp[1], pos[1])
+
+
+def test_a_slice_keeps_the_state_of_a_sequence_at_its_end():
+    """A sequence that reaches `max_positions` while another goes on: from then on its rows,
+    weights, positions and counts stay as they are, and the status says so at every step."""
+    from iquestrt_b200._lib import IqError
+    make, inputs = _slices(budget=40, keep_first=2, keep_last=10)
+    sl = make(max_positions=60)
+    sl.kv.set_lengths([39, 8])
+
+    def state():
+        kv = sl.kv
+        return [kv.held[:1].clone(), kv.seen[:1].clone()] + \
+            [x[0, :, :40].clone() for x in kv.weights + kv.positions] + \
+            [x[P.rows_of(kv.page_table, 0, 40, 16)].clone() for x in kv.k + kv.v]
+
+    for i in range(21):
+        sl.step(*inputs(i))
+        sl.check()
+    assert sl.kv.seen.tolist() == [60, 29] and sl.kv.held.tolist() == [40, 29]
+    before = state()
+    for i in range(21, 25):
+        sl.step(*inputs(i))
+        with pytest.raises(IqError):
+            sl.check()
+        assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip(before, state()))
+    assert sl.kv.seen.tolist() == [60, 33] and sl.kv.held.tolist() == [40, 33]
+    assert sl.kv.positions[1][1, 0, :33].tolist() == list(range(33))

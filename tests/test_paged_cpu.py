@@ -456,3 +456,16 @@ def test_rehearsal_puts_back_what_a_step_writes(budget, page):
             assert fail
         assert kv.page_table is table
         assert all(torch.equal(a, b) for a, b in zip(before, state()))
+
+
+def test_attention_slots_are_refused_without_weights():
+    from iquestrt_b200 import ops
+    L, lib, a = _attn_args()
+    a.slot = 4096
+    assert lib.iq_attn_decode(C.byref(a), None) == L.IQ_ERR_ARG
+    slot = torch.zeros(2, dtype=torch.int64)
+    w = torch.zeros(2, 2, 32)
+    for change, message in ((dict(slot=slot), "weights"), (dict(slot=slot[:1], weights=w), "shape"),
+                            (dict(slot=slot.int(), weights=w), "dtype")):
+        with pytest.raises(ValueError, match=message):
+            ops.attn_decode(**{**_tensors(), **change})

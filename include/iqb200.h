@@ -307,8 +307,9 @@ int iq_moe_down(const iq_moe_down_args* a, void* stream);
  * reach it, infinities and NaNs there included, nor do rows past lengths[b].  Softmax
  * statistics, scores and sums are fp32; the weights enter the product with v as half
  * precision (e4m3 caches) or bf16 (bf16 caches).  With e4m3 caches q enters its product as
- * half precision too, each row scaled by a power of two: exact but for elements some 2^30
- * below the row's largest.
+ * half precision too, each row scaled by the power of two that brings its largest element to
+ * [1, 2): elements down to 2^-17 of that power are exact, smaller ones off by at most 2^-25 of
+ * it.
  *
  * With `weights`, weights[b][h][j] gains the sum of the softmax weights that the query heads
  * and rows of key/value head h gave row j; for the step's own rows it is set to it, and

@@ -676,8 +676,9 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
         if (G::KV == IQ_ACT_BF16) {
           xs[nb][0] = xs[nb][1] = p.scale_log2;
         } else {
-          // bf16 values scaled by a power of two so that the row's largest lies in [1, 2):
-          // exact in half precision but for values 2^-14 below the row's largest
+          // bf16 values scaled by a power of two so that the row's largest lies in [1, 2): of
+          // eight significant bits, so exact in half precision (steps of 2^-24) down to 2^-17;
+          // smaller ones are rounded to that step, off by at most 2^-25
           float big = 0.f;
 #pragma unroll
           for (int x = 0; x < G::QREG; ++x)

@@ -494,7 +494,8 @@ def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, sca
     """Attention of the last `q_len` tokens of each sequence over its paged KV cache
     (`iq_attn_decode`): `q [batch, q_len, q_heads, D]` bf16 -> `out`, same shape.
 
-    `k_cache` / `v_cache [capacity, kv_heads, D]` are what `qkv_heads` writes (bf16 or e4m3),
+    `k_cache` / `v_cache [capacity, kv_heads, D]` are what `qkv_heads` writes (bf16, or e4m3,
+    with which each row of q is rounded to 2^-25 of its largest element or finer),
     row j of sequence b being row `page_table[b, j // page_size] * page_size + j % page_size`;
     `lengths [batch]` (int32) counts the rows with the new ones.  New token r sees the rows up
     to its own, the last `window` of them if `window` is not 0: rows of the cache, whose order

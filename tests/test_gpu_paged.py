@@ -816,3 +816,37 @@ def test_a_slice_keeps_the_state_of_a_sequence_at_its_end():
         assert all(torch.equal(_bits(a), _bits(b)) for a, b in zip(before, state()))
     assert sl.kv.seen.tolist() == [60, 33] and sl.kv.held.tolist() == [40, 33]
     assert sl.kv.positions[1][1, 0, :33].tolist() == list(range(33))
+
+
+@pytest.mark.parametrize("kv", [E4M3, BF16], ids=["e4m3", "bf16"])
+@pytest.mark.parametrize("down,heard", [(14, False), (14, True), (17, False), (20, False)])
+def test_elements_of_q_far_below_the_rows_largest(scratch, kv, heard, down):
+    """One channel of q lies some 2^`down` above the others, and the keys have something there
+    (`heard`) or zeros, so that the scores are the small elements' alone.  With e4m3 caches q is
+    rounded to 2^-25 of the power of two at or below the row's largest, here 1: a score is off by
+    that times scale sum |k| (beside what fp32 sums leave), a weight relative to the others by
+    twice that in the exponent; with bf16 caches q is taken as it is."""
+    from iquestrt_b200 import ops
+    lengths, d = [700, 40], 128
+    q, k, v, table, n = _case(lengths, 2, 8, 2, d, kv, 16, seed=23, sharp=2.0 ** -down)
+    q = q.clamp(-4 * 2.0 ** -down, 4 * 2.0 ** -down)
+    q[..., 5] = 1.0
+    if not heard:
+        k[..., 5] = 0.0
+    scale = 2.0 ** down * d ** -0.5
+    out = torch.full_like(q, float("nan"))
+    lse = torch.empty(q.shape[:3], device=DEV)
+    ops.attn_decode(q, k, v, table, n, page_size=16, scale=scale, out=out, lse=lse, scratch=scratch)
+    assert scratch.status() == 0
+    want = P.attn_decode(q, k, v, table, n, 16, scale=scale)
+    rows = torch.cat([P.rows_of(table, b, m, 16) for b, m in enumerate(lengths)])
+    step = scale * 2.0 ** -25 * float(k[rows].double().abs().sum(-1).max()) if kv == E4M3 else 0.0
+    score = (d + 2) * 2.0 ** -23 * want["reach"][..., None] + step
+    u = 2.0 ** -8 if kv == BF16 else 2.0 ** -11
+    rel = torch.expm1(2 * score) + u * (1 + torch.expm1(2 * score)) + 2.0 ** -21 + 2 * 700 * 2.0 ** -24
+    room = 1.01 * (2.0 ** -8 * want["out"].abs() + (1 + 2.0 ** -8) * rel * want["mass"]) + 6 * 700 * 2.0 ** -33
+    off = (out.double() - want["out"]).abs()
+    assert (off <= room).all(), float((off / room).max())
+    room = score[..., 0] + 2.0 ** -21 + 700 * 2.0 ** -24 + 2.0 ** -22 * want["lse"].abs()
+    off = (lse.double() - want["lse"]).abs()
+    assert (off <= room).all(), float((off / room).max())

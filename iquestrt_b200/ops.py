@@ -526,6 +526,7 @@ def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, sca
     _take("lengths", lengths, _I32, (batch,), index)
     if window < 0:
         raise ValueError(f"window must not be negative, got {window}")
+    window = min(window, page_size * pages)      # (more is no window, however much it is)
     if out is None:
         out = torch.empty(shape, dtype=_BF16, device=q.device)
     os_ = _take_out("out", out, _BF16, shape, index)

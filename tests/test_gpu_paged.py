@@ -850,3 +850,12 @@ def test_elements_of_q_far_below_the_rows_largest(scratch, kv, heard, down):
     room = score[..., 0] + 2.0 ** -21 + 700 * 2.0 ** -24 + 2.0 ** -22 * want["lse"].abs()
     off = (lse.double() - want["lse"]).abs()
     assert (off <= room).all(), float((off / room).max())
+
+
+@pytest.mark.parametrize("window", [112, 10 ** 6, 1 << 31, 1 << 62])
+def test_windows_past_the_page_table_are_none(scratch, window):
+    from iquestrt_b200 import ops
+    q, k, v, table, n = _case([100, 60], 2, 8, 2, 128, E4M3, 16, seed=52)
+    assert table.shape[1] * 16 == 112
+    want = ops.attn_decode(q, k, v, table, n, page_size=16, scratch=scratch)
+    assert torch.equal(ops.attn_decode(q, k, v, table, n, page_size=16, window=window, scratch=scratch), want)

@@ -859,3 +859,57 @@ def test_windows_past_the_page_table_are_none(scratch, window):
     assert table.shape[1] * 16 == 112
     want = ops.attn_decode(q, k, v, table, n, page_size=16, scratch=scratch)
     assert torch.equal(ops.attn_decode(q, k, v, table, n, page_size=16, window=window, scratch=scratch), want)
+
+
+@pytest.mark.parametrize("kv", [E4M3, BF16], ids=["e4m3", "bf16"])
+@pytest.mark.parametrize("d,page,q_len,qh", [(48, 16, 4, 8), (64, 3, 3, 8), (64, 64, 2, 4), (80, 64, 8, 16),
+                                             (128, 1, 4, 32), (192, 24, 2, 10), (256, 64, 4, 16)])
+@pytest.mark.parametrize("length", [90, 6000])
+def test_values_that_are_not_finite_stay_in_their_channel(scratch, kv, d, page, q_len, qh, length):
+    """Single NaNs and infinities among the values that only some rows of a step see (the newest
+    token's, one that slides out of the window), in sequences of one CTA and of many: the
+    channels of the rows and heads that see them get them, all else keeps its bits."""
+    from iquestrt_b200 import ops
+    window = 70 if length < 1000 else 5900
+    q, k, v, table, n = _case([length, 33], q_len, qh, 2, d, kv, page, seed=24)
+    call = dict(page_size=page, window=window, scratch=scratch)
+    clean = ops.attn_decode(q, k, v, table, n, **call).clone()
+    rows = P.rows_of(table, 0, length, page)
+    first, group = length - q_len - window + 1, qh // 2
+    bad = [(rows[-1], 0, 7, float("nan"), q_len - 1), (rows[-1], 1, d - 1, float("-inf"), q_len - 1),
+           (rows[first], 1, d // 2 + 1, float("inf"), 0), (rows[first], 0, 0, float("nan"), 0)]
+    want = clean.clone()
+    for row, h, c, x, r in bad:
+        if kv == E4M3:
+            x = float("nan")                     # (the type has no infinities)
+        v[row, h, c] = x
+        want[0, r, h * group:(h + 1) * group, c] = x
+    got = ops.attn_decode(q, k, v, table, n, **call)
+    assert scratch.status() == 0
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(got, nan=0.0), torch.nan_to_num(want, nan=0.0))
+
+
+@pytest.mark.parametrize("window", [0, 20])
+def test_slice_of_several_tokens_a_sequence_over_pages_of_its_own(window):
+    """Three sequences of two tokens a step, over a page table in any order with pages to spare:
+    every layer's attention of every step against 64 bits on what the cache held."""
+    g = _gen(99)
+    table = torch.randperm(20, generator=g, device=DEV).int()[:15].view(3, 5)
+    make, inputs = _slices(q_len=6, batch=3, rows=20, page_size=4, page_table=table, capacity=80)
+    sl = make(window=window)
+    sl.kv.set_lengths([10, 0, 3])
+    checked = []
+
+    def visit(layer, q, out, norm):
+        c = sl.kv
+        want = P.attn_decode(q.view(3, 2, 8, 128), c.k[layer], c.v[layer], table, c.lengths, 4,
+                             window=window)
+        _check(sl.attention.out.view(3, 2, 8, 128), None, want, E4M3, 128, 20)
+        checked.append(layer)
+
+    for i in range(5):
+        sl.step(*inputs(i), visit=visit)
+        sl.check()
+        assert sl.kv.held.tolist() == [12 + 2 * i, 2 + 2 * i, 5 + 2 * i]
+    assert checked == [0, 1] * 5

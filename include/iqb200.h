@@ -366,10 +366,12 @@ int iq_attn_decode(const iq_attn_args* a, void* stream);
  * to the lower row (a NaN weight counts as the lowest).  The rows that stay and lie below
  * `budget` keep their place; the others move into the freed places below it, the i-th such
  * row (ascending) into the i-th place.  From then on rows do not lie in the order of their
- * tokens (positions has it), so iq_attn_decode's window no longer means one.  K and V move in place; weights and positions of the
- * rows that stay go to weights_out / positions_out (which may be weights / positions
- * themselves, with their strides, but share no memory with them otherwise), entries from `budget` (or n) on are left as they were; lengths_out[b] = min(n,
- * budget) (not in the memory of `lengths` or `seen`: every head reads those).  Sequences must not share pages.
+ * tokens (positions has it), so iq_attn_decode's window no longer means one.  K and V move in
+ * place; weights and positions of the rows that stay go to weights_out / positions_out (which
+ * may be weights / positions themselves, with their strides, but share no memory with them
+ * otherwise), entries from `budget` (or n) on are left as they were; lengths_out[b] = min(n,
+ * budget) (not in the memory of `lengths` or `seen`: every head reads those).  Sequences must
+ * not share pages.
  *
  * Strides in elements, the caches' 16-byte aligned as in iq_attn_decode; rows = page_size *
  * max_pages up to 262144; `work` (iq_evict_work_bytes) needs no initialisation. */

@@ -35,10 +35,10 @@
 // the unit's keys get no weight, and their values are zeroed in shared memory first.
 //
 // Measured (one B200, both launches, pages of 64 unless said, 128 channels, 8 rows a head):
-// e4m3, 64 / 8 heads, 131071 keys: 51.0 us, 5.3 TB/s; 32768 keys, one 8 / 1 shard: 9.9 us;
+// e4m3, 64 / 8 heads, 131071 keys: 51.7 us, 5.2 TB/s; 32768 keys, one 8 / 1 shard: 9.9 us;
 // 32 sequences of 8192: 90 us, 6.0 TB/s; bf16, 48 sequences of 1 to 8192 keys, pages of 16:
-// 145 us, 6.3 TB/s (97 % of a copy's rate).  32 rows a head (four tokens) over 32k keys of
-// e4m3: 32.9 us, there the warp MMA and its feeding are the limit.  About 8 us of a call are
+// 146 us, 6.3 TB/s (96 % of a copy's rate).  32 rows a head (four tokens) over 32k keys of
+// e4m3: 32.8 us, there the warp MMA and its feeding are the limit.  About 8 us of a call are
 // fixed: two launches, the lengths -> page table -> keys chain, the joins.
 #include <math.h>
 #include <stdio.h>

@@ -143,7 +143,8 @@ class PagedKvCache:
         """What runs inside, on the current stream, leaves the cache as it was: the warm-up step
         before a capture.  The sequences hold nothing meanwhile, and the rows of the steps' first
         tokens are the caches' first ones for all of them, so that these rows are all there is
-        to put back (sequences that overwrite one another's change nothing but these)."""
+        to put back (sequences that overwrite one another's change nothing but these).  The
+        capture itself goes outside: inside, the page table is another."""
         table = self.page_table
         rows = min(self.q_len, self.page_size, self.capacity)
         kept = [self.held, self.lengths, self.seen, self.slot, self.pos]

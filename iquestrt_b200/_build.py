@@ -5,6 +5,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -64,11 +65,15 @@ def build(force: bool = False, verbose: bool = False) -> str:
         cmd = [nvcc, *NVCC_FLAGS, "-c", "-o", obj + new, os.path.join(CSRC, source)]
         if verbose:
             cmd[1:1] = ["-Xptxas", "-v"]
-        running.append((obj, subprocess.Popen(cmd, stdout=subprocess.PIPE,
-                                              stderr=subprocess.STDOUT, text=True)))
+        # (into a file: a pipe that fills up would hold its compiler until it is read)
+        out = tempfile.TemporaryFile("w+", errors="replace")
+        running.append((obj, out, subprocess.Popen(cmd, stdout=out, stderr=subprocess.STDOUT)))
     failed = []
-    for obj, proc in running:
-        text, _ = proc.communicate()
+    for obj, out, proc in running:
+        proc.wait()
+        out.seek(0)
+        text = out.read()
+        out.close()
         if proc.returncode != 0:
             failed.append(text)
             continue

@@ -820,17 +820,18 @@ __global__ void __launch_bounds__(G::THREADS, 1) attn_kernel(const __grid_consta
         const int jt = j0 + s0 * 16 + key_lo;
         float x[G::NBW][G::SUBI][4];
         auto masked = [&](int nb) {              // -infinity for what this lane's rows do not see
-          if (!EDGE) return;
+          if constexpr (EDGE) {
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int to = last_key[nb][y], from = p.window ? to - p.window : -1;
+            for (int y = 0; y < 2; ++y) {
+              const int to = last_key[nb][y], from = p.window ? to - p.window : -1;
 #pragma unroll
-            for (int sub = 0; sub < G::SUBI; ++sub)
+              for (int sub = 0; sub < G::SUBI; ++sub)
 #pragma unroll
-              for (int z = 0; z < 2; ++z) {
-                const int key = jt + sub * 16 + z * 8;
-                if (key <= from || key > to) x[nb][sub][2 * z + y] = -INFINITY;
-              }
+                for (int z = 0; z < 2; ++z) {
+                  const int key = jt + sub * 16 + z * 8;
+                  if (key <= from || key > to) x[nb][sub][2 * z + y] = -INFINITY;
+                }
+            }
           }
         };
         if (SCORES && (!EDGE || p.scores)) {

@@ -58,6 +58,7 @@ class Scratch:
         self.bytes = int(lib.iq_scratch_bytes())
         self.buf = torch.zeros(self.bytes, dtype=torch.uint8, device=device)
         self.ptr = self.buf.data_ptr()
+        self.index = self.buf.get_device()
 
     def status(self, clear: bool = True) -> int:
         """Synchronises the current stream and returns the device status code.  After an
@@ -468,6 +469,15 @@ def _gpu(name, index):
         raise ValueError(f"{name} must be a CUDA tensor")
 
 
+def _status(scratch, index):
+    """Address of the status word; a kernel that finds an error writes there."""
+    if scratch is None:
+        return 0
+    if scratch.index != index:
+        raise ValueError(f"scratch must be on cuda:{index}, got {scratch.buf.device}")
+    return scratch.ptr
+
+
 class AttnWork:
     """The work area of `attn_decode` for given sizes (`rows`: page_size x pages of the page
     table; `weights`: for calls that accumulate weights).  Calls that share one must be
@@ -567,7 +577,7 @@ def attn_decode(q, k_cache, v_cache, page_table, lengths, *, page_size: int, sca
         lengths.data_ptr(), batch, q_len, q_heads, kv_heads, d, window,
         d ** -0.5 if scale is None else scale, out.data_ptr(), os_[0], os_[1], os_[2], lse_ptr,
         w_ptr, ws[0], ws[1], w_rows, pos_ptr, ps[0], ps[1], seen_ptr, slot_ptr, work.ptr, work.bytes,
-        0 if scratch is None else scratch.ptr, int(pdl)))
+        _status(scratch, index), int(pdl)))
     return out
 
 
@@ -635,7 +645,7 @@ def kv_evict(k_cache, v_cache, page_table, lengths, weights, positions, seen, *,
         page_table.data_ptr(), ts, page_size, pages, n_ptr, seen.data_ptr(), weights.data_ptr(),
         ws[0], ws[1], positions.data_ptr(), ps[0], ps[1], weights_out.data_ptr(), wo[0], wo[1],
         positions_out.data_ptr(), po[0], po[1], out_ptr, batch, kv_heads, d, budget, keep_first,
-        keep_last, work.ptr, work.bytes, 0 if scratch is None else scratch.ptr, int(pdl)))
+        keep_last, work.ptr, work.bytes, _status(scratch, index), int(pdl)))
     return lengths_out
 
 
@@ -670,5 +680,5 @@ def kv_advance(page_table, lengths, seen, slot, pos, *, page_size: int, capacity
     _on(index, "iq_kv_advance", _lib.PACK_ADVANCE.pack(
         page_table.data_ptr(), ts, page_size, pages, capacity, lengths.data_ptr(), seen.data_ptr(),
         lengths_out.data_ptr(), seen_out.data_ptr(), slot.data_ptr(), pos.data_ptr(), batch, q_len,
-        max_positions, 0 if scratch is None else scratch.ptr, int(pdl)))
+        max_positions, _status(scratch, index), int(pdl)))
     return slot, pos

@@ -913,3 +913,23 @@ def test_slice_of_several_tokens_a_sequence_over_pages_of_its_own(window):
         sl.check()
         assert sl.kv.held.tolist() == [12 + 2 * i, 2 + 2 * i, 5 + 2 * i]
     assert checked == [0, 1] * 5
+
+
+def test_a_scratch_of_another_device_is_refused():
+    """Its status word would be written from this device."""
+    from iquestrt_b200 import ops
+    other = ops.Scratch("cpu")
+    q, k, v, table, n = _case([40, 3], 1, 8, 2, 128, E4M3, 16, seed=53)
+    w = torch.zeros(2, 2, table.shape[1] * 16, device=DEV)
+    pos = torch.zeros_like(w, dtype=torch.int32)
+    slot = torch.zeros(2, dtype=torch.int64, device=DEV)
+    before = n.clone()
+    calls = [lambda: ops.attn_decode(q, k, v, table, n, page_size=16, scratch=other),
+             lambda: ops.kv_evict(k, v, table, n, w, pos, n, page_size=16, budget=8,
+                                  lengths_out=n.clone(), scratch=other),
+             lambda: ops.kv_advance(table, n, n.clone(), slot, slot.clone(), page_size=16,
+                                    capacity=k.shape[0], scratch=other)]
+    for call in calls:
+        with pytest.raises(ValueError, match="scratch must be on cuda:0"):
+            call()
+    assert torch.equal(n, before)
